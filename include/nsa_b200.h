@@ -224,6 +224,18 @@ int nsa_window_attn_bwd(const void* q, const void* k, const void* v, const void*
                         int total_len, int batch, int max_seqlen, int num_q_heads, int num_kv_heads, int head_dim,
                         int window_left, const long long* strides, float sm_scale, int dtype, void* stream);
 
+/* Sliding window with sinks: query t of a sequence sees key j <= t iff t - j <= window_left or j < num_sinks.  No counterpart in the
+ * reference.  Tensors, strides and lse convention as nsa_window_attn_fwd / nsa_window_attn_bwd, head_dim 64 or 128; no bound on the lengths
+ * is needed.  Output, dq, dk and dv of rows behind the last sequence are zero.  Workspace: nsa_sink_window_attn_bwd_workspace bytes. */
+int nsa_sink_window_attn_fwd(const void* q, const void* k, const void* v, const int* cu_seqlens, void* o, float* lse, int total_len,
+                             int batch, int num_q_heads, int num_kv_heads, int head_dim, int window_left, int num_sinks,
+                             const long long* strides, float sm_scale, int dtype, void* stream);
+long long nsa_sink_window_attn_bwd_workspace(int total_len, int num_q_heads, int num_kv_heads, int head_dim);
+int nsa_sink_window_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse,
+                             const int* cu_seqlens, void* dq, void* dk, void* dv, void* workspace, long long workspace_bytes,
+                             int total_len, int batch, int num_q_heads, int num_kv_heads, int head_dim, int window_left, int num_sinks,
+                             const long long* strides, float sm_scale, int dtype, void* stream);
+
 /* Bytes of scratch nsa_topk_sparse_attn_bwd needs (fp32 dk/dv accumulators, (lse, delta) pairs, inverted index). */
 long long nsa_topk_sparse_attn_bwd_workspace(int total_len, int batch, int num_q_heads, int num_kv_heads,
                                              int head_dim, int topk, int block_size);
@@ -386,6 +398,42 @@ int nsa_decode_step_supported(int batch, int num_q_heads, int num_kv_heads, int 
 int nsa_linear_decode_taps(const void* k, const void* v, const void* w_k, const void* w_v, const void* pe,
                            const void* stage_cache, const int* stage_len, float* taps, int batch, int num_kv_heads, int head_dim, int kernel_size,
                            int kernel_stride, const long long* strides, int dtype, void* stream);
+
+/* ---- paged key-value cache (no counterpart in the reference) ----
+ * k_pages, v_pages [num_pages, page_size, num_kv_heads, d] (any strides of multiples of 8 elements, d contiguous); row j of sequence b is
+ * slot j % page_size of page block_table[b][j / page_size], block_table int32 [batch, max_pages].  Entries behind a sequence's rows are not
+ * read.  A page number outside [0, num_pages), or a length above page_size * max_pages, raises device status 2; its rows are not touched. */
+
+/* Writes rows of k, v [total_len, num_kv_heads, d] behind the seqlens[b] rows that sequence b holds: rows cu_seqlens[b] .. cu_seqlens[b + 1],
+ * or (cu_seqlens NULL, total_len = batch) one row each.  seqlens_after[b] (another buffer than seqlens): the length after that, at most
+ * page_size * max_pages.  strides[11]: k_n k_h | v_n v_h | (page, slot, head) of k_pages, v_pages | block_table row. */
+int nsa_paged_kv_append(void* k_pages, void* v_pages, const int* block_table, const int* seqlens, const void* k, const void* v,
+                        const int* cu_seqlens, int* seqlens_after, int total_len, int batch, int num_kv_heads, int head_dim,
+                        int num_pages, int page_size, int max_pages, const long long* strides, void* stream);
+
+/* One query token per sequence, at the position of the last of its seqlens[b] rows, attends to row j iff window_left < 0 (all rows), or
+ * seqlens[b] - 1 - j <= window_left, or j < num_sinks.  q, o [batch, num_q_heads, d]; a sequence without rows gets zeros.  weights float
+ * [batch, num_kv_heads, >= page_size * max_pages] or NULL: the probabilities of a row, summed over the heads of its group, are added.
+ * Groups of up to 16 query heads.  scratch: nsa_paged_decode_scratch_floats(batch, num_q_heads, d, page_size * max_pages, weights != NULL)
+ * floats, of which the first nsa_paged_decode_control_words() are zero before the first call and left at zero.
+ * strides[13]: q_b q_h | (page, slot, head) of k_pages, v_pages | o_b o_h | block_table row | weights_b weights_h. */
+long long nsa_paged_decode_control_words(void);
+long long nsa_paged_decode_scratch_floats(int batch, int num_q_heads, int head_dim, int capacity, int with_weights);
+int nsa_paged_attn_decode(const void* q, const void* k_pages, const void* v_pages, const int* block_table, const int* seqlens, void* o,
+                          float* weights, float* scratch, long long scratch_floats, int batch, int num_q_heads, int num_kv_heads,
+                          int head_dim, int num_pages, int page_size, int max_pages, int window_left, int num_sinks,
+                          const long long* strides, float sm_scale, int dtype, void* stream);
+
+/* Keeps min(seqlens[b], budget) rows of every sequence and KV head: where there are more, the first num_sinks, the last num_recent and the
+ * others with the largest weights (equal ones: the lower row; one that is no number counts as the smallest), and writes them in their order
+ * to the pages of new_block_table [batch, max_new_pages], which hold no row of block_table's sequences.  kept int32 [batch, num_kv_heads,
+ * budget]: their old rows, -1 behind; weights_after float [batch, num_kv_heads, weight_columns]: their weights, 0 behind; seqlens_after
+ * [batch].  weights: rows of at least page_size * max_pages floats.
+ * strides[10]: weights_b weights_h | (page, slot, head) of k_pages, v_pages | rows of block_table, new_block_table. */
+int nsa_paged_kv_evict(void* k_pages, void* v_pages, const int* block_table, const int* seqlens, const float* weights,
+                       const int* new_block_table, int* seqlens_after, float* weights_after, int* kept, int batch, int num_kv_heads,
+                       int head_dim, int num_pages, int page_size, int max_pages, int max_new_pages, int weight_columns, int budget,
+                       int num_sinks, int num_recent, const long long* strides, void* stream);
 
 #ifdef __cplusplus
 }

@@ -36,6 +36,11 @@ _SIGNATURES = {
     "nsa_pool_compress_fwd": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _L, _L, _I, _P],
     "nsa_varlen_attn_bwd": [_P] * 12 + [_L] + [_I] * 11 + [_P, _F, _I, _P],
     "nsa_window_attn_bwd": [_P] * 11 + [_L] + [_I] * 7 + [_P, _F, _I, _P],
+    "nsa_sink_window_attn_fwd": [_P] * 6 + [_I] * 7 + [_P, _F, _I, _P],
+    "nsa_sink_window_attn_bwd": [_P] * 11 + [_L] + [_I] * 7 + [_P, _F, _I, _P],
+    "nsa_paged_kv_append": [_P] * 8 + [_I] * 7 + [_P, _P],
+    "nsa_paged_attn_decode": [_P] * 8 + [_L] + [_I] * 9 + [_P, _F, _I, _P],
+    "nsa_paged_kv_evict": [_P] * 9 + [_I] * 10 + [_P, _P],
     "nsa_topk_sparse_attn_bwd": [_P] * 13 + [_L] + [_I] * 7 + [_P, _F, _I, _P],
     "nsa_linear_compress_bwd": [_P] * 10 + [_I] * 8 + [_L, _L, _I, _P],
     "nsa_pool_compress_bwd": [_P] * 10 + [_L] + [_I] * 8 + [_L, _L, _I, _P],
@@ -66,6 +71,9 @@ _SIZE_QUERIES = {
     "nsa_pool_compress_bwd_workspace_floats": [_I] * 7,
     "nsa_varlen_attn_bwd_workspace": [_I, _I, _I, _I, _I],
     "nsa_varlen_attn_bwd_workspace_one_pass": [_I, _I, _I, _I, _I, _I, _I],
+    "nsa_sink_window_attn_bwd_workspace": [_I, _I, _I, _I],
+    "nsa_paged_decode_control_words": [],
+    "nsa_paged_decode_scratch_floats": [_I, _I, _I, _I, _I],
     "nsa_topk_sparse_attn_bwd_workspace": [_I, _I, _I, _I, _I, _I, _I],
     "nsa_launch_count": [],
     "nsa_flash_attn_decode_static_capacity": [],

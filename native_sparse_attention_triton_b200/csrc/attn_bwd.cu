@@ -23,6 +23,8 @@
 #include "host_util.h"
 #include "nsa_b200.h"
 #include "attn_bwd.h"
+#include "sink_exact.cuh"
+#include "work_steal.cuh"
 
 namespace nsa {
 
@@ -821,6 +823,90 @@ static int run_dense_bwd(const void* q, const void* k, const void* v, const void
   return cv.run<T>(stream);
 }
 
+// Tokens per CTA of the dK/dV pass of a window with sinks, in row tiles of 128 / G tokens: all that see a key tile where that leaves two
+// CTAs for every SM.
+static int sink_chunk(int total, int batch, int Hkv, int G, int left) {
+  const int per = 128 / G;
+  const long long tiles = (total / 128ll + batch) * Hkv;
+  const int span = std::min<long long>(total, (long long)left + 128);
+  int chunk = std::min(64, (span + per - 1) / per);
+  while (chunk > 4 && tiles * ((span + chunk * per - 1) / (chunk * per)) < 2 * 148) chunk = (chunk + 1) / 2;
+  return chunk * per;
+}
+
+// fp32 sums of dK and dV -> storage type; a warp per row of a head.  Rows with a value that is not finite are computed one by one.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) sink_finish_kernel(DkdvParams p, const __grid_constant__ SinkMaps maps, void* dk, void* dv, long long dk_sn,
+                                                          long long dk_sh, long long dv_sn, long long dv_sh, int rows) {
+  const long long x = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (x >= (long long)rows * p.Hkv) return;
+  const int n = (int)(x / p.Hkv), h = (int)(x % p.Hkv), lane = lane_id();
+  float4 a, b;
+  if constexpr (D == 128) {
+    a = __ldcs(reinterpret_cast<const float4*>(p.dk32 + x * D) + lane);
+    b = __ldcs(reinterpret_cast<const float4*>(p.dv32 + x * D) + lane);
+  } else {
+    const float2 a2 = __ldcs(reinterpret_cast<const float2*>(p.dk32 + x * D) + lane), b2 = __ldcs(reinterpret_cast<const float2*>(p.dv32 + x * D) + lane);
+    a = make_float4(a2.x, a2.y, 0.f, 0.f);
+    b = make_float4(b2.x, b2.y, 0.f, 0.f);
+  }
+  const float top = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))), fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w))));
+  const bool nan = a.x != a.x || a.y != a.y || a.z != a.z || a.w != a.w || b.x != b.x || b.y != b.y || b.z != b.z || b.w != b.w;
+  if (__any_sync(0xffffffffu, nan || top == INFINITY) && n < __ldg(p.cu_q + p.B)) {
+    const int s = find_sequence(p.cu_q, p.B, n), row0 = __ldg(p.cu_q + s);
+    exact_key_row<T, D>(a, b, &maps, p.ld, p.Hq, row0, __ldg(p.cu_q + s + 1) - row0, n - row0, h, p.G, p.left, p.sinks, p.scale2, p.sm_scale);
+  }
+  store_lane_elements<T, D>(static_cast<T*>(dk) + n * dk_sn + h * dk_sh, a);
+  store_lane_elements<T, D>(static_cast<T*>(dv) + n * dv_sn + h * dv_sh, b);
+}
+
+template <typename T, int D>
+static int run_sink_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, const int* cu, void* dq,
+                        void* dk, void* dv, void* ws, int total, int batch, int Hq, int Hkv, int left, int sinks, const long long* S, float sm_scale,
+                        cudaStream_t stream) {
+  const int G = Hq / Hkv;
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  float2* ld = reinterpret_cast<float2*>(w);
+  w += align_up((size_t)total * Hq * sizeof(float2), 256);
+  float* dk32 = reinterpret_cast<float*>(w);
+  w += align_up((size_t)total * Hkv * D * sizeof(float), 256);
+  float* dv32 = reinterpret_cast<float*>(w);
+  w += align_up((size_t)total * Hkv * D * sizeof(float), 256);
+  cudaError_t e = cudaMemsetAsync(dk32, 0, w - reinterpret_cast<uint8_t*>(dk32), stream);
+  if (e != cudaSuccess) return cuda_rc(e);
+  DenseBwdParams p;
+  p.q = q; p.o = o; p.dout = dout; p.lse = lse; p.ld = ld; p.dq = dq; p.cu_q = cu; p.cu_k = cu;
+  p.q_sn = S[0]; p.q_sh = S[1]; p.o_sn = S[6]; p.o_sh = S[7]; p.do_sn = S[8]; p.do_sh = S[9]; p.dq_sn = S[10]; p.dq_sh = S[11];
+  p.B = batch; p.Hq = Hq; p.Hkv = Hkv; p.G = G;
+  p.logG = 0;
+  while ((1 << p.logG) < G) ++p.logG;
+  p.window = 1; p.stride = 1; p.causal = 1; p.left = left; p.sinks = sinks;
+  p.scale2 = sm_scale * kLog2e; p.sm_scale = sm_scale;
+  p.st.word = status_word();
+  const int dt = DT<T>::kTmapType == CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 ? NSA_DTYPE_BF16 : NSA_DTYPE_FP16;
+  int rc = dense_dq_tc(k, v, S[2], S[3], S[4], S[5], total, total, total, D, dt, p, stream);
+  if (rc) return rc;
+  DkdvParams d;
+  d.ld = ld; d.dk32 = dk32; d.dv32 = dv32; d.cu_q = cu; d.cu_k = cu;
+  d.offsets = nullptr; d.item_base = nullptr; d.item_bin = nullptr; d.item_counter = nullptr; d.list = nullptr;
+  d.B = batch; d.Hq = Hq; d.Hkv = Hkv; d.G = G; d.TB = 0; d.NW = 1; d.block_size = kKeyTile;
+  d.window = 1; d.stride = 1; d.causal = 1; d.left = left; d.sinks = sinks;
+  d.scale2 = p.scale2; d.sm_scale = sm_scale; d.st = p.st;
+  d.chunk = sink_chunk(total, batch, Hkv, G, left);
+  d.key_slots = (int)row_tile_slots(total, batch, 7);
+  d.sink_log = 13 - p.logG;  // 64 row tiles
+  while (d.sink_log > 9 - p.logG && row_tile_slots(total, batch, d.sink_log) * Hkv < 148) --d.sink_log;
+  const long long ds[8] = {S[0], S[1], S[2], S[3], S[4], S[5], S[8], S[9]};
+  rc = launch_dense_dkdv_tc<T, D>(q, dout, k, v, ds, total, total, (int)std::min<long long>(total, (long long)left + 128), 0, batch, d, stream);
+  if (rc) return rc;
+  SinkMaps maps;
+  rc = make_sink_maps(maps, DT<T>::kTmapType, q, k, v, dout, ds, D, Hkv, total, sinks);
+  if (rc) return rc;
+  LaunchScope ls_("sink_finish", stream);
+  sink_finish_kernel<T, D><<<(unsigned)(((long long)total * Hkv + 7) / 8), 256, 0, stream>>>(d, maps, dk, dv, S[12], S[13], S[14], S[15], total);
+  return cuda_rc(cudaGetLastError());
+}
+
 // dQ comes out of the tcgen05 dK/dV pass for these groups; the others have the mma.sync passes.
 static bool sparse_fused_dq(int G) { return G >= 4 && (G & (G - 1)) == 0; }
 
@@ -1023,6 +1109,29 @@ extern "C" int nsa_window_attn_bwd(const void* q, const void* k, const void* v, 
   return varlen_attn_bwd_common(q, k, v, o, dout, lse, cu_seqlens, cu_seqlens, dq, dk, dv, workspace, workspace_bytes, total_len,
                                 total_len, batch, max_seqlen, max_seqlen, num_q_heads, num_kv_heads, head_dim, 1, 1, 1,
                                 window_left, strides, sm_scale, dtype, stream);
+}
+
+extern "C" long long nsa_sink_window_attn_bwd_workspace(int total_len, int num_q_heads, int num_kv_heads, int head_dim) {
+  return (long long)nsa::dense_ws_bytes(total_len, total_len, num_q_heads, num_kv_heads, head_dim);
+}
+
+extern "C" int nsa_sink_window_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse,
+                                        const int* cu_seqlens, void* dq, void* dk, void* dv, void* workspace, long long workspace_bytes,
+                                        int total_len, int batch, int num_q_heads, int num_kv_heads, int head_dim, int window_left,
+                                        int num_sinks, const long long* strides, float sm_scale, int dtype, void* stream) {
+  using namespace nsa;
+  if (!q || !k || !v || !o || !dout || !lse || !cu_seqlens || !dq || !dk || !dv || !workspace || !strides) return kInvalid;
+  if (total_len <= 0 || batch <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || window_left < 0 || num_sinks < 0) return kInvalid;
+  const int G = num_q_heads / num_kv_heads;
+  if (G > 16 || G < 1 || (G & (G - 1))) return kUnsupported;
+  for (int i = 0; i < 16; ++i)
+    if (strides[i] % 8) return kInvalid;
+  for (const void* rows : {q, k, v, o, dout, (const void*)dq, (const void*)dk, (const void*)dv})  // read and written 16 bytes at a time
+    if (!aligned16(rows)) return kInvalid;
+  if (workspace_bytes < nsa_sink_window_attn_bwd_workspace(total_len, num_q_heads, num_kv_heads, head_dim)) return kWorkspace;
+  return NSA_DISPATCH_T_D(dtype, head_dim, run_sink_bwd, q, k, v, o, dout, lse, cu_seqlens, dq, dk, dv, workspace, total_len, batch, num_q_heads,
+                          num_kv_heads, std::min(window_left, total_len), std::min(num_sinks, total_len), strides, sm_scale,
+                          static_cast<cudaStream_t>(stream));
 }
 
 extern "C" long long nsa_topk_sparse_attn_bwd_workspace(int total_len, int batch, int num_q_heads, int num_kv_heads,

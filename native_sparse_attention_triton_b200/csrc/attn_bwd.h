@@ -46,6 +46,9 @@ struct DkdvParams {
   int left;  // dense dK/dV pass only; >= 0: sliding window (key >= t - left, plain causal mask), < 0: none
   float scale2, sm_scale;
   Status st;
+  // sliding window with sinks (key < sinks seen by all later tokens); sinks < 0: none.  The grid's first `key_slots` places stand for
+  // key tiles, the others for the sinks' key tiles and 2^sink_log tokens each.
+  int sinks = -1, key_slots = 0, sink_log = 0;
 };
 
 
@@ -65,7 +68,14 @@ struct DenseBwdParams {
   int left;  // >= 0: sliding window (key >= t - left, plain causal mask), < 0: none
   float scale2, sm_scale;
   Status st;
+  int sinks = -1;  // >= 0: sliding window with sinks (... or key < sinks)
+  int rows = 0;    // of dq
 };
+
+struct SinkMaps;
+// strides S: q_n q_h k_n k_h v_n v_h do_n do_h (the last two where dout is given)
+int make_sink_maps(SinkMaps& m, CUtensorMapDataType dt, const void* q, const void* k, const void* v, const void* dout, const long long* S, int D,
+                   int Hkv, int Nk, int sinks);
 
 // tcgen05 implementation of the dense dQ pass (dense_dq_tc.cu).  k/v strides in elements.
 int dense_dq_tc(const void* k, const void* v, long long k_sn, long long k_sh, long long v_sn, long long v_sh, int total_q,

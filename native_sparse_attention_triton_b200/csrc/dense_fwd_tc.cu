@@ -35,6 +35,8 @@
 #include "dispatch.h"
 #include "host_util.h"
 #include "nsa_b200.h"
+#include "sink_exact.cuh"
+#include "sink_keys.cuh"
 #include "tc5.cuh"
 #include "work_steal.cuh"
 
@@ -56,6 +58,8 @@ struct DenseFwdTcParams {
   int left;  // >= 0: sliding window, a query also needs key >= t - left (plain causal mask only); < 0: no lower bound
   float scale2;
   Status st;
+  int sinks;  // SINKS: ... or key < sinks
+  int rows;   // SINKS: of the output
 };
 
 __device__ __forceinline__ int visible_keys_tc(int t, int Lk, int window, int stride, int causal) {
@@ -70,10 +74,12 @@ constexpr int kTcQBufs = 3;         // row tiles of Q
 constexpr int kTcSoftWarps = 8;     // 4 per row tile
 constexpr int kTcThreads = (kTcSoftWarps + 3) * 32;
 
-template <typename T, int D>
+// SINKS: a sliding window with sinks; an item's key tiles are those of its list of keys (sink_keys.cuh), whose shift stands in the item's kt0.
+template <typename T, int D, bool SINKS>
 __global__ void __launch_bounds__(kTcThreads, 1)
 dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, DenseFwdTcParams p) {
+                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, DenseFwdTcParams p,
+                    const __grid_constant__ TileMaps<SINKS> split) {
   constexpr int PANELS = D / 64;
   constexpr int PANEL_BYTES = 128 * 128;            // 128 rows x 128 B
   constexpr int Q_BYTES = 128 * D * 2;              // one row tile
@@ -140,6 +146,7 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     int kt = 0;    // key tiles so far
     auto lookup = [&](uint3 blk, AttnItem& w) {
       int b, tile;
+      if constexpr (SINKS) zero_rows_behind<T, D>(p.o, p.o_sn, p.o_sh, __ldg(p.cu_q + p.B), p.rows, blk.x, gridDim.x, blk.y * p.G, p.G);
       // long rows first
       if (!find_row_tile(p.cu_q, p.B, 8 - p.logG, (int)gridDim.x - 1 - (int)blk.x, b, w.qs, w.Lq, tile)) return false;
       w.head = blk.y;
@@ -147,6 +154,11 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       w.Lk = __ldg(p.cu_k + b + 1) - w.ksq;
       w.q0 = tile * 2 * QT;
       const int t_hi = min(w.q0 + 2 * QT, w.Lq) - 1;
+      if constexpr (SINKS) {
+        w.kt0 = sink_shift(w.q0, p.left, sink_room(p.sinks));
+        w.ntiles = (t_hi + 1 - w.kt0 + kTcKeyTile - 1) / kTcKeyTile;
+        return true;
+      }
       // with a sliding window the first key tiles are invisible to every row of the item: start at tile kt0
       w.kt0 = p.left >= 0 ? max(0, w.q0 - p.left) / kTcKeyTile : 0;
       w.ntiles = max(0, (visible_keys_tc(t_hi, w.Lk, p.window, p.stride, p.causal) + kTcKeyTile - 1) / kTcKeyTile - w.kt0);
@@ -167,6 +179,10 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           const int c = kt + i, s = c % kTcStages;
           if (c >= kTcStages) mbar_wait(empty + s, ((c / kTcStages) - 1) & 1, p.st);
           mbar_expect_tx(full + s, KV_BYTES);
+          if constexpr (SINKS) {
+            load_key_tile<PANELS, PANEL_BYTES>(sm + s * KV_BYTES, tm, tm == &tmK ? split.k : split.v, full + s, w.head, w.ksq, i, sink_room(p.sinks), w.kt0);
+            return;
+          }
 #pragma unroll
           for (int pn = 0; pn < PANELS; ++pn)
             tma_load_3d(sm + s * KV_BYTES + pn * PANEL_BYTES, tm, full + s, pn * 64, w.head, w.ksq + (w.kt0 + i) * kTcKeyTile);
@@ -225,6 +241,11 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       }
     };
     auto q_tile = [&](unsigned t) { return q_base + t % kTcQBufs * Q_BYTES; };
+    // V of tile i of the present item, in stage st, before its products
+    auto clean_v = [&](unsigned st, int i) {
+      if constexpr (SINKS)
+        clean_key_tile<PANELS, PANEL_BYTES>(v_base + st * KV_BYTES, i, min(w.q0 + 2 * QT, w.Lq) - w.kt0, p.sinks, w.kt0);
+    };
     // S of tile x of the item that starts at row tile t, for its first key tile c
     auto start = [&](unsigned c, unsigned t, int x) {
       if (x == 0) mbar_wait(k_full + c % kTcStages, (c / kTcStages) & 1, p.st);
@@ -248,6 +269,7 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       for (int i = 0; i + 1 < ntiles; ++i, ++c) {
         const unsigned n = c + 1;
         mbar_wait(v_full + c % kTcStages, (c / kTcStages) & 1, p.st);
+        clean_v(c % kTcStages, i);
         mbar_wait(k_full + n % kTcStages, (n / kTcStages) & 1, p.st);
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
@@ -265,7 +287,10 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 #pragma unroll 1
       for (int g = 0; g < 2; ++g) {
         mbar_wait(p_full + g, c & 1, p.st);
-        if (g == 0) mbar_wait(v_full + c % kTcStages, (c / kTcStages) & 1, p.st);
+        if (g == 0) {
+          mbar_wait(v_full + c % kTcStages, (c / kTcStages) & 1, p.st);
+          clean_v(c % kTcStages, ntiles - 1);
+        }
         tc_fence_after_sync();
         issue_pv(c % kTcStages, g, ntiles == 1);
         if (have < 0) have = next_item(g == 1);
@@ -316,11 +341,13 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       for (int i = 0; i < ntiles; ++i) {
         mbar_wait(s_full + g, (kt + i) & 1, p.st);
         tc_fence_after_sync();
-        const int lim = nvis - (w.kt0 + i) * kTcKeyTile;  // columns below lim are visible ...
-        const int lo = p.left >= 0 ? tpos - p.left - (w.kt0 + i) * kTcKeyTile : 0;  // ... from column lo on
+        const int col0 = SINKS ? w.kt0 + i * kTcKeyTile : (w.kt0 + i) * kTcKeyTile;  // key of column 0, in the window
+        const int lim = nvis - col0;  // columns below lim are visible ...
+        const int lo = SINKS || p.left >= 0 ? tpos - p.left - col0 : 0;  // ... from column lo on
+        const int sink = SINKS ? min(p.sinks, nvis) - i * kTcKeyTile : 0;  // ... and those below sink
         // Key tiles that every row of the warp sees in full (all but those on the mask's edge) take a path without the
         // per-element mask instructions.
-        const bool full = __all_sync(0xffffffffu, lim >= kTcKeyTile && lo <= 0);
+        const bool full = __all_sync(0xffffffffu, lim >= kTcKeyTile && lo <= (SINKS ? max(sink, 0) : 0));
         // Full tiles of rows that already have a reference maximum are tried in ONE pass over the logits: exponentials
         // relative to the current reference, with the maximum of the exponents tracked on the side.  If no row of the
         // warp outgrew its reference by more than 2^8 -- the same test the general form makes -- the packed P is stored
@@ -366,7 +393,12 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           // raised) reference.
           auto seen = [&](int c) {
             const int hi_c = min(32, max(0, lim - c * 32)), lo_c = min(32, max(0, lo - c * 32));
-            return (hi_c < 32 ? (1u << hi_c) - 1u : 0xffffffffu) & ~(lo_c < 32 ? (1u << lo_c) - 1u : 0xffffffffu);
+            const uint32_t in = (hi_c < 32 ? (1u << hi_c) - 1u : 0xffffffffu) & ~(lo_c < 32 ? (1u << lo_c) - 1u : 0xffffffffu);
+            if constexpr (SINKS) {
+              const int sk = min(32, max(0, sink - c * 32));
+              return in | (sk < 32 ? (1u << sk) - 1u : 0xffffffffu);
+            }
+            return in;
           };
           float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -493,6 +525,23 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           *reinterpret_cast<uint4*>(orow + ci * 8) = out;
         }
       }
+      if constexpr (SINKS) {
+        // rows with a value that is not finite, one by one
+        bool fine = true;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) fine = fine && fabsf(__uint_as_float(r[c][j])) < INFINITY;
+        __syncwarp();
+        for (unsigned redo = __ballot_sync(0xffffffffu, valid && !fine); redo; redo &= redo - 1) {
+          const int src = __ffs(redo) - 1;
+          const int t = __shfl_sync(0xffffffffu, tpos, src), hd = __shfl_sync(0xffffffffu, head, src), rw = __shfl_sync(0xffffffffu, row, src);
+          const float ls = __shfl_sync(0xffffffffu, m_ref + log2f(l), src);
+          const float4 x = exact_query_row<T, D, false>(&split, w.qs, t, hd, w.head, p.left, p.sinks, p.scale2, 0.f, ls, 0.f);
+          if (staged) store_lane_elements_swizzled<T, D, PANEL_BYTES>(q_sm + qb * Q_BYTES, rw, x);
+          else store_lane_elements<T, D>(static_cast<T*>(p.o) + (long long)(w.qs + t) * p.o_sn + (long long)hd * p.o_sh, x);
+        }
+      }
       if (ntiles > 0) {
         if (staged) fence_proxy_async();  // the TMA engine reads the tile through the async proxy
         __syncwarp();
@@ -507,7 +556,22 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   if (warp == kTcSoftWarps + 1) tmem_dealloc(tmem, 512);
 }
 
-template <typename T, int D>
+// The two boxes of a split tile of K and V (none where the sinks fill whole tiles).
+int make_sink_maps(SinkMaps& m, CUtensorMapDataType dt, const void* q, const void* k, const void* v, const void* dout, const long long* S, int D,
+                   int Hkv, int Nk, int sinks) {
+  m.q = q; m.keys = k; m.values = v; m.dout = dout;
+  m.q_sn = S[0]; m.q_sh = S[1]; m.k_sn = S[2]; m.k_sh = S[3]; m.v_sn = S[4]; m.v_sh = S[5]; m.do_sn = S[6]; m.do_sh = S[7];
+  const int first = sink_room(sinks) % 128;
+  for (int x = 0; x < 2; ++x) {
+    const int rows = first == 0 ? 128 : x ? 128 - first : first;
+    int rc = make_tmap_3d(&m.k[x], dt, k, D, Hkv, Nk, S[3], S[2], 64, 1, rows);
+    if (!rc) rc = make_tmap_3d(&m.v[x], dt, v, D, Hkv, Nk, S[5], S[4], 64, 1, rows);
+    if (rc) return rc;
+  }
+  return kOk;
+}
+
+template <typename T, int D, bool SINKS>
 static int launch_dense_fwd_tc(const void* q, const void* k, const void* v, const long long* S, int Nq, int Nk, DenseFwdTcParams p, cudaStream_t stream) {
   // S: q_n q_h k_n k_h v_n v_h o_n o_h
   CUtensorMap tmQ, tmK, tmV;
@@ -522,28 +586,38 @@ static int launch_dense_fwd_tc(const void* q, const void* k, const void* v, cons
   rc = make_tmap_3d(&tmO, DT<T>::kTmapType, p.o, D, p.Hq, Nq, p.o_sh, p.o_sn, 64, p.G, QT);
   if (rc) return rc;
   const size_t smem = (kTcQBufs + 2 * kTcStages) * 128 * D * 2 + sizeof(StealSlot) + sizeof(ItemRing) + 24 * sizeof(uint64_t);
-  auto kern = dense_fwd_tc_kernel<T, D>;
+  TileMaps<SINKS> split;
+  if constexpr (SINKS) {
+    rc = make_sink_maps(split, DT<T>::kTmapType, q, k, v, nullptr, S, D, p.Hkv, Nk, p.sinks);
+    if (rc) return rc;
+  }
+  auto kern = dense_fwd_tc_kernel<T, D, SINKS>;
   cudaError_t e = allow_smem(kern, smem);
   if (e != cudaSuccess) return cuda_rc(e);
   const dim3 grid((unsigned)row_tile_slots(Nq, p.B, 8 - p.logG), p.Hkv);
-  { LaunchScope ls_("dense_fwd_tc", stream); kern<<<grid, kTcThreads, smem, stream>>>(tmQ, tmK, tmV, tmO, p); }
+  { LaunchScope ls_(SINKS ? "sink_fwd_tc" : "dense_fwd_tc", stream); kern<<<grid, kTcThreads, smem, stream>>>(tmQ, tmK, tmV, tmO, p, split); }
   return cuda_rc(cudaGetLastError());
 }
 
-// entry used by nsa_varlen_attn_fwd (dense_fwd.cu)
+template <typename T, int D>
+static int launch_dense(const void* q, const void* k, const void* v, const long long* S, int Nq, int Nk, DenseFwdTcParams p, cudaStream_t stream) {
+  return p.sinks < 0 ? launch_dense_fwd_tc<T, D, false>(q, k, v, S, Nq, Nk, p, stream) : launch_dense_fwd_tc<T, D, true>(q, k, v, S, Nq, Nk, p, stream);
+}
+
+// entry used by nsa_varlen_attn_fwd (dense_fwd.cu) and, with sinks >= 0, by nsa_sink_window_attn_fwd
 int varlen_attn_fwd_tc(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, void* o, float* lse,
                        int total_q, int total_k, int batch, int Hq, int Hkv, int head_dim, int causal,
-                       int window, int stride, int left, const long long* strides, float sm_scale, int dtype, cudaStream_t stream) {
+                       int window, int stride, int left, int sinks, const long long* strides, float sm_scale, int dtype, cudaStream_t stream) {
   DenseFwdTcParams p;
   p.o = o; p.lse = lse; p.cu_q = cu_q; p.cu_k = cu_k;
   p.o_sn = strides[6]; p.o_sh = strides[7];
   p.B = batch; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
   p.logG = 0;
   while ((1 << p.logG) < p.G) ++p.logG;
-  p.window = window; p.stride = stride; p.causal = causal; p.left = left;
+  p.window = window; p.stride = stride; p.causal = causal; p.left = left; p.sinks = sinks; p.rows = total_q;
   p.scale2 = sm_scale * kLog2e;
   p.st.word = status_word();
-  return NSA_DISPATCH_T_D(dtype, head_dim, launch_dense_fwd_tc, q, k, v, strides, total_q, total_k, p, stream);
+  return NSA_DISPATCH_T_D(dtype, head_dim, launch_dense, q, k, v, strides, total_q, total_k, p, stream);
 }
 
 }  // namespace nsa

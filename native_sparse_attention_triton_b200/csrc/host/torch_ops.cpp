@@ -67,6 +67,12 @@ void require_cuda(const Tensor& t, const Ts&... more) {
   require_cuda(more...);
 }
 
+template <typename... Ts>
+void one_device(const Tensor& first, const Ts&... more) {
+  require_cuda(first, more...);
+  for (const Tensor* t : {&more...}) NSA_ASSERT(t->device() == first.device(), "all tensors must be on one device");
+}
+
 bool is_16bit(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }
 int dtype_code(const Tensor& t) {
   if (t.scalar_type() == at::kBFloat16) return NSA_DTYPE_BF16;
@@ -550,6 +556,85 @@ Tensor sliding_window_attention(const Tensor& q, const Tensor& k, const Tensor& 
                                    sm_scale.value_or(default_scale(q.size(2)))}).o;
 }
 
+// ----------------------------------------------------------------------------------------- sliding window with sinks
+struct SinkWindowBackward final : SavingNode {
+  int left, sinks;
+  double scale;
+  std::string name() const override { return "SinkWindowAttentionBackward"; }
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(3);
+    if (!grads[0].defined()) return out;
+    const auto s = unpack();
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const Tensor &q = s[0], &k = s[1], &v = s[2], &o = s[3], &lse = s[4], &cu = s[5];
+    const int64_t N = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = k.size(1);
+    for (int i = 0; i < 3; ++i) out[i] = empty_like_rows(s[i]);
+    if (N == 0) return out;
+    const Tensor dout = gradient_rows(grads[0]);
+    const long long bytes = nsa_sink_window_attn_bwd_workspace((int)N, (int)Hq, (int)Hkv, (int)D);
+    Tensor ws = empty({bytes}, at::kByte, q.device());
+    QkvStrides st;
+    st.add(q).add(k).add(v).add(o).add(dout).add(out[0]).add(out[1]).add(out[2]);
+    Launch run(q);
+    check_rc(nsa_sink_window_attn_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(dout), ptr<float>(lse), ptr<int>(cu), ptr(out[0]), ptr(out[1]), ptr(out[2]),
+                                      ptr(ws), bytes, (int)N, (int)cu.size(0) - 1, (int)Hq, (int)Hkv, (int)D, left, sinks, st.s, (float)scale,
+                                      dtype_code(q), run.stream),
+             "nsa_sink_window_attn_bwd");
+    return out;
+  }
+};
+
+Tensor sink_window_attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& cu, int64_t window, int64_t sinks,
+                             std::optional<double> sm_scale) {
+  NSA_ASSERT(q_in.dim() == 3 && k_in.dim() == 3 && v_in.dim() == 3, "q, k and v must be [total_len, num_heads, head_dim]");
+  check_qkv_dtypes(q_in, k_in, v_in);
+  NSA_ASSERT(is_int32(cu) && cu.dim() == 1 && cu.size(0) >= 2 && cu.is_contiguous(), "cu_seqlens must be a contiguous int32 vector of batch + 1 entries");
+  NSA_ASSERT(k_in.sizes() == v_in.sizes(), "k and v must have the same shape");
+  NSA_ASSERT(q_in.size(0) == k_in.size(0) && q_in.size(2) == k_in.size(2), "q, k and v need as many rows, of the same head_dim");
+  NSA_ASSERT(k_in.size(1) > 0 && q_in.size(1) > 0 && q_in.size(1) % k_in.size(1) == 0, "query heads must be a multiple of the key/value heads");
+  NSA_ASSERT(q_in.size(2) == 64 || q_in.size(2) == 128, "sink_window_attention supports head_dim 64 and 128");
+  const int64_t G = q_in.size(1) / k_in.size(1);
+  if (G > 16 || (G & (G - 1)))
+    raise_python(PyExc_NotImplementedError, "query heads per key/value head must be a power of two of at most 16");
+  NSA_ASSERT(window >= 0 && sinks >= 0, "window_size and num_sinks must not be negative");
+  NSA_ASSERT(q_in.size(0) < INT_MAX / 2, "at most 2^30 rows");
+  const double scale = sm_scale.value_or(default_scale(q_in.size(2)));
+  NSA_ASSERT(scale > 0 && std::isfinite(scale), "sm_scale must be positive");
+  one_device(q_in, k_in, v_in, cu);
+  const bool graph = needs_graph({q_in, k_in, v_in});
+  const int left = (int)std::min<int64_t>(window, INT_MAX / 2), s = (int)std::min<int64_t>(sinks, INT_MAX / 2);
+  Tensor q, k, v, o, lse;
+  {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    q = inner_contiguous(q_in);
+    k = inner_contiguous(k_in);
+    v = inner_contiguous(v_in);
+    const int64_t N = q.size(0), Hq = q.size(1), D = q.size(2);
+    o = empty({N, Hq, D}, q.scalar_type(), q.device());
+    lse = empty({N, Hq}, at::kFloat, q.device());
+    if (N > 0) {
+      QkvStrides st;
+      st.add(q).add(k).add(v).add(o);
+      Launch run(q);
+      check_rc(nsa_sink_window_attn_fwd(ptr(q), ptr(k), ptr(v), ptr<int>(cu), ptr(o), ptr<float>(lse), (int)N, (int)cu.size(0) - 1, (int)Hq,
+                                        (int)k.size(1), (int)D, left, s, st.s, (float)scale, dtype_code(q), run.stream),
+               "nsa_sink_window_attn_fwd");
+    }
+  }
+  if (graph) {
+    auto node = make_node<SinkWindowBackward>(q_in, k_in, v_in);
+    node->left = left;
+    node->sinks = s;
+    node->scale = scale;
+    torch::autograd::set_history(o, node);
+    for (const Tensor& t : {q, k, v}) node->saved.push_back(save_input(t));
+    node->saved.push_back(SavedVariable(o, /*is_output=*/true));
+    for (const Tensor& t : {lse, cu}) node->saved.push_back(save_input(t));
+  }
+  return o;
+}
+
 // --------------------------------------------------------------------------------------------- selected-block attention
 struct SparseAttentionBackward final : SavingNode {
   int block_size;
@@ -886,6 +971,147 @@ std::tuple<Tensor, Tensor> compressed_attention_decode(const Tensor& q_in, const
   return {o, idx};
 }
 
+// ------------------------------------------------------------------------------------------------------------ paged cache
+// What the three paged operators ask of a cache: k_pages, v_pages [pages, page_size, heads, d], block_table int32 [batch, columns].
+struct Pages {
+  int64_t pages, page, heads, d, columns, batch, capacity;
+};
+Pages check_pages(const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& seqlens, const char* table_name = "block_table") {
+  NSA_ASSERT(k.dim() == 4 && v.dim() == 4 && k.sizes() == v.sizes(), "k_pages and v_pages must be [num_pages, page_size, num_kv_heads, head_dim]");
+  NSA_ASSERT(is_16bit(k) && k.scalar_type() == v.scalar_type(), "k_pages and v_pages must be of one type, bfloat16 or float16");
+  NSA_ASSERT(k.size(3) == 64 || k.size(3) == 128, "paged operators support head_dim 64 and 128");
+  NSA_ASSERT(k.numel() > 0, "the cache must have pages");
+  NSA_ASSERT(is_int32(table) && table.dim() == 2 && table.size(1) > 0 && (table.stride(1) == 1 || table.size(1) == 1),
+             "block_table must be int32 [batch, max_pages] with contiguous rows");
+  NSA_ASSERT(is_int32(seqlens) && seqlens.dim() == 1 && seqlens.is_contiguous(), "seqlens must be a contiguous int32 vector");
+  NSA_ASSERT(seqlens.size(0) == table.size(0), "seqlens and block_table need an entry for every sequence");
+  const Pages p{k.size(0), k.size(1), k.size(2), k.size(3), table.size(1), table.size(0), k.size(1) * table.size(1)};
+  NSA_ASSERT(p.pages < INT_MAX && p.capacity <= (1 << 30) && p.batch * p.heads <= (1 << 30), "at most 2^30 rows in a sequence and 2^30 (sequence, head) pairs");
+  for (const Tensor* t : {&k, &v}) {
+    bool ok = t->stride(3) == 1 && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && t->stride(i) % 8 == 0;
+    NSA_ASSERT(ok, "k_pages and v_pages need contiguous head_dim, 16-byte aligned rows (a cache is never copied)");
+  }
+  return p;
+}
+// A tensor that is written in place.
+void check_written(const Tensor& t) {
+  NSA_ASSERT(!(at::GradMode::is_enabled() && t.requires_grad()), "a tensor that is written in place must not require gradients");
+  at::assert_no_internal_overlap(t);
+}
+void wrote(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+Tensor paged_kv_append(const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& seqlens, const Tensor& k_in, const Tensor& v_in,
+                       const OptTensor& cu) {
+  const Pages c = check_pages(kp, vp, table, seqlens);
+  NSA_ASSERT(k_in.dim() == 3 && k_in.sizes() == v_in.sizes() && k_in.size(1) == c.heads && k_in.size(2) == c.d,
+             "k and v must be [rows, num_kv_heads, head_dim] of the cache");
+  NSA_ASSERT(k_in.scalar_type() == kp.scalar_type() && v_in.scalar_type() == kp.scalar_type(), "k and v must have the cache's dtype");
+  NSA_ASSERT(k_in.size(0) < INT_MAX / 2, "at most 2^30 rows");
+  if (cu) {
+    NSA_ASSERT(is_int32(*cu) && cu->dim() == 1 && cu->is_contiguous() && cu->size(0) == c.batch + 1, "cu_seqlens must be a contiguous int32 vector of batch + 1 entries");
+  } else {
+    NSA_ASSERT(k_in.size(0) == c.batch, "without cu_seqlens there is one row per sequence");
+  }
+  one_device(kp, vp, table, seqlens, k_in, v_in);
+  if (cu) one_device(kp, *cu);
+  check_written(kp);
+  check_written(vp);
+  at::NoGradGuard no_grad;
+  at::AutoDispatchBelowADInplaceOrView guard;
+  const Tensor k = inner_contiguous(k_in), v = inner_contiguous(v_in);
+  Tensor after = empty({c.batch}, at::kInt, kp.device());
+  if (c.batch == 0) return after;
+  const long long st[11] = {k.stride(0), k.stride(1), v.stride(0), v.stride(1), kp.stride(0), kp.stride(1), kp.stride(2), vp.stride(0), vp.stride(1),
+                            vp.stride(2), table.stride(0)};
+  Launch run(kp);
+  check_rc(nsa_paged_kv_append(ptr(kp), ptr(vp), ptr<int>(table), ptr<int>(seqlens), ptr(k), ptr(v), static_cast<int*>(ptr(cu)), ptr<int>(after),
+                               (int)k.size(0), (int)c.batch, (int)c.heads, (int)c.d, (int)c.pages, (int)c.page, (int)c.columns, st, run.stream),
+           "nsa_paged_kv_append");
+  wrote(kp);
+  wrote(vp);
+  return after;
+}
+
+Tensor paged_attention_decode(const Tensor& q_in, const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& seqlens,
+                              std::optional<double> sm_scale, std::optional<int64_t> window, int64_t sinks, const OptTensor& weights) {
+  const Pages c = check_pages(kp, vp, table, seqlens);
+  NSA_ASSERT(q_in.dim() == 3 && q_in.size(0) == c.batch && q_in.size(2) == c.d, "q must be [batch, num_q_heads, head_dim] of the cache");
+  NSA_ASSERT(q_in.scalar_type() == kp.scalar_type(), "q must have the cache's dtype");
+  NSA_ASSERT(q_in.size(1) > 0 && q_in.size(1) % c.heads == 0, "query heads must be a multiple of the key/value heads");
+  if (q_in.size(1) / c.heads > 16) raise_python(PyExc_NotImplementedError, "at most 16 query heads per key/value head");
+  NSA_ASSERT(!window || *window >= 0, "window_size must not be negative");
+  NSA_ASSERT(sinks >= 0, "num_sinks must not be negative");
+  const double scale = sm_scale.value_or(default_scale(c.d));
+  NSA_ASSERT(std::isfinite(scale), "sm_scale must be finite");
+  if (weights)
+    NSA_ASSERT(weights->scalar_type() == at::kFloat && weights->dim() == 3 && weights->size(0) == c.batch && weights->size(1) == c.heads &&
+                   weights->size(2) >= c.capacity && weights->stride(2) == 1,
+               "weights must be float32 [batch, num_kv_heads, max_pages * page_size or more] with contiguous rows");
+  one_device(kp, vp, table, seqlens, q_in);
+  if (weights) {
+    one_device(kp, *weights);
+    check_written(*weights);
+  }
+  at::NoGradGuard no_grad;
+  at::AutoDispatchBelowADInplaceOrView guard;
+  const Tensor q = inner_contiguous(q_in);
+  Tensor o = empty_like_rows(q);
+  if (c.batch == 0) return o;
+  const long long st[13] = {q.stride(0), q.stride(1), kp.stride(0), kp.stride(1), kp.stride(2), vp.stride(0), vp.stride(1), vp.stride(2), o.stride(0),
+                            o.stride(1), table.stride(0), weights ? weights->stride(0) : 0, weights ? weights->stride(1) : 0};
+  const int left = window ? (int)std::min<int64_t>(*window, INT_MAX / 2) : -1, s = (int)std::min<int64_t>(sinks, INT_MAX / 2);
+  Launch run(q);
+  const long long n = nsa_paged_decode_scratch_floats((int)c.batch, (int)q.size(1), (int)c.d, (int)c.capacity, weights.has_value());
+  const uint64_t key = scratch_key(q.device(), c10::cuda::getCurrentCUDAStream(q.device().index()));
+  const Tensor buf = take_scratch(nsa_paged_decode_control_words() - 1, n, q.device(), key);
+  const int rc = nsa_paged_attn_decode(ptr(q), ptr(kp), ptr(vp), ptr<int>(table), ptr<int>(seqlens), ptr(o), weights ? ptr<float>(*weights) : nullptr,
+                                       ptr<float>(buf), n, (int)c.batch, (int)q.size(1), (int)c.heads, (int)c.d, (int)c.pages, (int)c.page,
+                                       (int)c.columns, left, s, st, (float)scale, dtype_code(q), run.stream);
+  if (rc) {  // a failed call may have left control words that are not zero
+    std::lock_guard<std::mutex> lk(g_scratch_mu);
+    g_scratch.erase(key);
+  }
+  check_rc(rc, "nsa_paged_attn_decode");
+  if (weights) wrote(*weights);
+  return o;
+}
+
+std::tuple<Tensor, Tensor, Tensor> paged_kv_evict(const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& seqlens, const Tensor& weights,
+                                                  const Tensor& target, int64_t budget, int64_t sinks, int64_t recent) {
+  const Pages c = check_pages(kp, vp, table, seqlens);
+  NSA_ASSERT(is_int32(target) && target.dim() == 2 && target.size(0) == c.batch && target.size(1) > 0 && (target.stride(1) == 1 || target.size(1) == 1),
+             "new_block_table must be int32 [batch, max_new_pages] with contiguous rows");
+  NSA_ASSERT(weights.scalar_type() == at::kFloat && weights.dim() == 3 && weights.size(0) == c.batch && weights.size(1) == c.heads &&
+                 weights.size(2) >= c.capacity && weights.stride(2) == 1 && weights.size(2) < INT_MAX,
+             "weights must be float32 [batch, num_kv_heads, max_pages * page_size or more] with contiguous rows");
+  NSA_ASSERT(budget > 0 && budget <= (1 << 30), "budget must be positive, at most 2^30");
+  NSA_ASSERT(sinks >= 0 && recent >= 0 && sinks <= budget && recent <= budget - sinks, "num_sinks and num_recent must fit into the budget");
+  NSA_ASSERT(target.size(1) * c.page <= (1 << 30), "at most 2^30 rows in a sequence");
+  NSA_ASSERT(target.size(1) * c.page >= std::min<int64_t>(budget, c.capacity), "new_block_table must have room for the rows that are kept");
+  one_device(kp, vp, table, seqlens, weights, target);
+  NSA_ASSERT(table.data_ptr() != target.data_ptr() || c.batch == 0, "new_block_table must name other pages than block_table");
+  check_written(kp);
+  check_written(vp);
+  at::NoGradGuard no_grad;
+  at::AutoDispatchBelowADInplaceOrView guard;
+  Tensor after = empty({c.batch}, at::kInt, kp.device()), kept = empty({c.batch, c.heads, budget}, at::kInt, kp.device()),
+         sums = empty(weights.sizes(), at::kFloat, kp.device());
+  if (c.batch == 0) return {after, sums, kept};
+  const long long st[10] = {weights.stride(0), weights.stride(1), kp.stride(0), kp.stride(1), kp.stride(2), vp.stride(0), vp.stride(1), vp.stride(2),
+                            table.stride(0), target.stride(0)};
+  Launch run(kp);
+  check_rc(nsa_paged_kv_evict(ptr(kp), ptr(vp), ptr<int>(table), ptr<int>(seqlens), ptr<float>(weights), ptr<int>(target), ptr<int>(after),
+                              ptr<float>(sums), ptr<int>(kept), (int)c.batch, (int)c.heads, (int)c.d, (int)c.pages, (int)c.page, (int)c.columns,
+                              (int)target.size(1), (int)weights.size(2), (int)budget, (int)sinks, (int)recent, st, run.stream),
+           "nsa_paged_kv_evict");
+  wrote(kp);
+  wrote(vp);
+  return {after, sums, kept};
+}
+
 // ------------------------------------------------------------------------------------------------------- inference step
 // The caches of a layer as NSACache holds them: [2, batch, rows, heads, d] tensors and int32 counters.
 struct CacheRefs {
@@ -1017,12 +1243,16 @@ PYBIND11_MODULE(_nsa_host, m) {
   m.def("compressed_attention", &compressed_attention);
   m.def("flash_attention_varlen", &flash_attention_varlen);
   m.def("sliding_window_attention", &sliding_window_attention);
+  m.def("sink_window_attention", &sink_window_attention);
   m.def("topk_sparse_attention", &topk_sparse_attention);
   m.def("gate_combine", &gate_combine);
   m.def("rope", &rope);
   m.def("flash_attention_decode", &flash_attention_decode);
   m.def("topk_sparse_attention_decode", &topk_sparse_attention_decode);
   m.def("compressed_attention_decode", &compressed_attention_decode);
+  m.def("paged_kv_append", &paged_kv_append);
+  m.def("paged_attention_decode", &paged_attention_decode);
+  m.def("paged_kv_evict", &paged_kv_evict);
   m.def("decode_step", &decode_step);
   m.def("prefill", &prefill);
 }

@@ -135,6 +135,18 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 // TMEM address of (lane, column) relative to an allocation base
 __device__ __forceinline__ uint32_t tmem_addr(uint32_t base, int lane, int col) { return base + ((uint32_t)lane << 16) + (uint32_t)col; }
 
+// Rows [from, to) of an operand tile of PANELS panels set to zero, by a whole warp, in front of the products that read it: what TMA
+// brought there may be another sequence's row or nobody's, and a masked probability of 0 does not hide one that is not finite.
+template <int PANELS, int PANEL>
+__device__ __forceinline__ void zero_tile_rows(uint32_t tile, int from, int to) {
+#pragma unroll
+  for (int pn = 0; pn < PANELS; ++pn)
+    for (int c = from * 8 + lane_id(); c < to * 8; c += 32)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(tile + pn * PANEL + c * 16), "r"(0) : "memory");
+  fence_proxy_async();  // the tensor core reads it through the async proxy
+  __syncwarp();
+}
+
 __device__ __forceinline__ bool elect_one() {
   uint32_t pred;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(pred));

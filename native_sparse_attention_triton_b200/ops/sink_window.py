@@ -1,0 +1,22 @@
+"""Causal varlen attention with a sliding window and sinks: the first keys of a sequence stay visible to all its queries.
+
+The reference has no operator for it; it stands next to sliding_window_attention, whose call it takes without max_seqlen.  Its
+single-token form is paged_attention_decode with window_size and num_sinks.
+"""
+from typing import Optional
+
+import torch
+
+from .. import _lib
+
+
+def sink_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, window_size: int, num_sinks: int,
+                          sm_scale: Optional[float] = None) -> torch.Tensor:
+    """q [total, Hq, d], k/v [total, Hkv, d] (self-attention: one cu_seqlens, int32 [batch + 1]); key j of a sequence is visible to its
+    query i iff j <= i and (i - j <= window_size or j < num_sinks).
+
+    bfloat16 or float16, head_dim 64 or 128, Hq / Hkv a power of two of at most 16 (NotImplementedError otherwise).  Differentiable in q, k
+    and v.  Rows behind the last sequence (a padded batch) may hold anything: they reach no other row, and their output and gradients are
+    zero.  A value that is not finite reaches the rows that see it and no others.
+    """
+    return _lib.host().sink_window_attention(q, k, v, cu_seqlens, int(window_size), int(num_sinks), sm_scale)

@@ -986,7 +986,8 @@ Pages check_pages(const Tensor& k, const Tensor& v, const Tensor& table, const T
   NSA_ASSERT(is_int32(seqlens) && seqlens.dim() == 1 && seqlens.is_contiguous(), "seqlens must be a contiguous int32 vector");
   NSA_ASSERT(seqlens.size(0) == table.size(0), "seqlens and block_table need an entry for every sequence");
   const Pages p{k.size(0), k.size(1), k.size(2), k.size(3), table.size(1), table.size(0), k.size(1) * table.size(1)};
-  NSA_ASSERT(p.pages < INT_MAX && p.capacity <= (1 << 30) && p.batch * p.heads <= (1 << 30), "at most 2^30 rows in a sequence and 2^30 (sequence, head) pairs");
+  NSA_ASSERT(p.pages < INT_MAX && p.capacity <= (1 << 30) && p.batch * p.heads <= (1 << 30) && (double)p.batch * p.heads * (p.capacity + 31) < 0x1p36,
+             "at most 2^30 rows in a sequence, and 2^36 rows in block_table for all sequences and heads");
   for (const Tensor* t : {&k, &v}) {
     bool ok = t->stride(3) == 1 && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0;
     for (int i = 0; i < 3; ++i) ok = ok && t->stride(i) % 8 == 0;

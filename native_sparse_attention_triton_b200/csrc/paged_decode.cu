@@ -4,17 +4,16 @@
 //     j < L  and  (no window, or j >= L - 1 - window, or j < sinks),
 // which is what the query at position L - 1 sees in the varlen form (sink_window_attention).  For every query head
 //     o = sum_j p_j v_j,   p_j = 2^(x_j - m) / l,   x_j = scale log2(e) <q, k_j>,   m = max x_j,   l = sum_j 2^(x_j - m).
-// Row j lies in page table[b][j / page], slot j % page.  The visible rows are counted without the gap between the sinks and the
-// window, so that neither costs a tile of masked keys.
+// Row j lies in page table[b][j / page], slot j % page.
 //
 // What bounds it is HBM: 4 D bytes of K and V per visible row and KV head against 4 D G flops, which 16 x 8 x 16 products of one warp
 // (rows = the G query heads of a KV head) take with room to spare.
 //
-// The tiles of all (sequence, KV head) pairs form one list, which is cut evenly over the CTAs and their warps whatever the lengths are:
-// a warp walks a run of tiles that may end one pair and begin others.  It gathers tiles of kTileRows rows with cp.async, a row's address
-// from its page, into a ring of its own, keeps a running maximum and sum and writes a pair that lies in its run whole.  Parts of a pair
+// A sequence's rows are cut into tiles of 32; those with a visible row, of all (sequence, KV head) pairs, form one list, which is
+// cut evenly over the CTAs and their warps whatever the lengths are: a warp walks a run of tiles that may end one pair and begin others.
+// It fetches them into a ring of its own, keeps a running maximum and sum and writes a pair that lies in its run whole.  Parts of a pair
 // are joined in the order of the list, within a CTA through shared memory and between CTAs through scratch, by the CTA that finishes
-// last: the result does not depend on who that is.
+// last: the result does not depend on which one that is.
 //
 // The probabilities are rounded to 16 bits twice, p = hi + lo, for two products instead of one: their rounding (2^-9 in bf16, as much as
 // the output's own) then costs nothing that can be seen, and the products are not what bounds the kernel.
@@ -24,13 +23,21 @@
 #include "nsa_b200.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace nsa {
 
 namespace {
-constexpr int kPagedWarps = 4;
+constexpr int kPagedRows = 32;  // of a tile: one a lane
 constexpr int kPagedStages = 3;
-constexpr int kPagedTileBytes = 32 * 128 * 2;  // of K, and of V: 32 rows of 128 elements or 64 of 64
+// Warps and shared memory of a CTA, one an SM: 192 KB of rings either way.
+template <int D>
+struct PagedShape {
+  static constexpr int kWarps = D == 128 ? 4 : 8;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kTileBytes = kPagedRows * D * 2;           // of K, and of V
+  static constexpr int kRing = kPagedStages * 2 * kTileBytes;     // of a warp
+};
 }  // namespace
 
 struct PagedDecodeParams {
@@ -40,95 +47,127 @@ struct PagedDecodeParams {
   void* o;
   const int* table;
   const int* seqlens;
-  float* logits;  // [pairs][G][cap] base-2 logits by visible row, or nullptr
+  float* logits;  // [pairs][G][cap] base-2 logits by row, or nullptr
   float* lse;     // [pairs][G], with logits
   unsigned* ctrl;
   float* part;    // [CTAs][2][16][D + 2]
   long long q_sb, q_sh, k_sp, k_ss, k_sh, v_sp, v_ss, v_sh, o_sb, o_sh, t_sb;
   int B, Hkv, G, page, max_pages, num_pages, cap;
+  int box;            // rows of a TMA box: they divide a page and a tile
   int window, sinks;  // window < 0: every row
   float scale2;
   Status st;
 };
 
-// Visible rows of a sequence: [0, gap_at) and [gap_at + gap, gap + n).
+// Visible rows of a sequence, [0, head) and [first, len); its tiles, [0, gap_at) and [gap_at + gap, gap_at + gap + ...), n of them.
 struct Rows {
-  int n, gap_at, gap;
+  int len, head, first, n, gap_at, gap;
 };
-__device__ __forceinline__ Rows visible_rows(int len, int window, int sinks, int cap) {
+__device__ __forceinline__ Rows visible_rows(const PagedDecodeParams& p, int b) {
+  constexpr int R = kPagedRows;
   Rows r;
-  len = max(0, min(len, cap));
-  const int first = window < 0 ? 0 : max(0, len - 1 - window);
-  r.gap_at = min(sinks, first);
-  r.gap = first - r.gap_at;
-  r.n = len - r.gap;
+  r.len = max(0, min(__ldg(p.seqlens + b), p.cap));
+  r.first = p.window < 0 ? 0 : max(0, r.len - 1 - p.window);
+  r.head = min(p.sinks, r.first);
+  r.gap_at = min((r.head + R - 1) / R, r.first / R);
+  r.gap = r.first / R - r.gap_at;
+  r.n = max(1, (r.len + R - 1) / R - r.gap);  // a sequence without rows has a tile of which none is visible
   return r;
 }
 
 // A position in the list of tiles.
-template <int ROWS>
 struct TileCursor {
-  int b, h, t, ntiles;
+  int b, h, t;
   Rows rows;
-  __device__ __forceinline__ void load(const PagedDecodeParams& p) {
-    rows = visible_rows(__ldg(p.seqlens + b), p.window, p.sinks, p.cap);
-    ntiles = max(1, (rows.n + ROWS - 1) / ROWS);
-  }
+  __device__ __forceinline__ int row0() const { return (t < rows.gap_at ? t : t + rows.gap) * kPagedRows; }
   __device__ __forceinline__ void next(const PagedDecodeParams& p) {
-    if (++t < ntiles) return;
+    if (++t < rows.n) return;
     t = 0;
     if (++h < p.Hkv) return;
     h = 0;
-    if (++b < p.B) load(p);
+    if (++b < p.B) rows = visible_rows(p, b);
   }
 };
 
-template <int ROWS>
-__device__ __forceinline__ int tiles_of(const PagedDecodeParams& p, int b) {
-  return max(1, (visible_rows(__ldg(p.seqlens + b), p.window, p.sinks, p.cap).n + ROWS - 1) / ROWS);
-}
-
-// Tiles of the whole list.  A whole warp.
-template <int ROWS>
-__device__ __forceinline__ long long count_tiles(const PagedDecodeParams& p) {
-  long long sum = 0;
-  for (int b = lane_id(); b < p.B; b += 32) {
-    sum += tiles_of<ROWS>(p, b);
+// The tiles in front of every THREADS-th part of the batch, in `before`; returns those of the whole list.  The whole CTA.
+template <int THREADS>
+__device__ __forceinline__ unsigned count_tiles(const PagedDecodeParams& p, unsigned* before, unsigned* warp_sums) {
+  const int per = (p.B + THREADS - 1) / THREADS, b0 = min(p.B, (int)threadIdx.x * per), b1 = min(p.B, b0 + per);
+  unsigned sum = 0;
+  for (int b = b0; b < b1; ++b) {
+    sum += visible_rows(p, b).n;
     if (blockIdx.x == 0 && __ldg(p.seqlens + b) > p.cap) p.st.raise(kErrBadIndex);  // more rows than its pages hold
   }
+  sum *= p.Hkv;
+  unsigned upto = sum;
 #pragma unroll
-  for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-  return sum * p.Hkv;
+  for (int s = 1; s < 32; s <<= 1) {
+    const unsigned y = __shfl_up_sync(0xffffffffu, upto, s);
+    if (lane_id() >= s) upto += y;
+  }
+  if (lane_id() == 31) warp_sums[threadIdx.x >> 5] = upto;
+  __syncthreads();
+  unsigned total = 0, front = upto - sum;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    const unsigned x = warp_sums[w];
+    front += w < (int)(threadIdx.x >> 5) ? x : 0;
+    total += x;
+  }
+  before[threadIdx.x] = front;
+  __syncthreads();
+  return total;
 }
 
 // The cursor of tile number x.  A whole warp.
-template <int ROWS>
-__device__ __forceinline__ TileCursor<ROWS> find_tile(const PagedDecodeParams& p, long long x) {
-  TileCursor<ROWS> c;
-  long long before = 0;
-  for (int b0 = 0;; b0 += 32) {
-    const int b = b0 + lane_id();
-    const int mine = b < p.B ? tiles_of<ROWS>(p, b) : 0;
-    long long upto = (long long)mine * p.Hkv;
+template <int THREADS>
+__device__ __forceinline__ TileCursor find_tile(const PagedDecodeParams& p, const unsigned* before, unsigned x) {
+  const int per = (p.B + THREADS - 1) / THREADS, lane = lane_id();
+  int part = -1;
+#pragma unroll
+  for (int k = 0; k < THREADS / 32; ++k) part += __popc(__ballot_sync(0xffffffffu, before[k * 32 + lane] <= x));
+  TileCursor c;
+  unsigned at = x - before[part];
+  const int end = min(p.B, (part + 1) * per);
+  for (int b0 = part * per;; b0 += 32) {
+    const int b = b0 + lane;
+    const unsigned mine = b < end ? visible_rows(p, b).n * p.Hkv : 0;
+    unsigned upto = mine;
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, upto, s);
-      if (lane_id() >= s) upto += y;
+      const unsigned y = __shfl_up_sync(0xffffffffu, upto, s);
+      if (lane >= s) upto += y;
     }
-    const unsigned past = __ballot_sync(0xffffffffu, before + upto > x);
-    if (past || b0 + 32 >= p.B) {
+    const unsigned past = __ballot_sync(0xffffffffu, upto > at);
+    if (past || b0 + 32 >= end) {
       const int src = past ? __ffs(past) - 1 : 31;
-      const long long start = before + __shfl_sync(0xffffffffu, upto, src) - (long long)__shfl_sync(0xffffffffu, mine, src) * p.Hkv;
+      at -= __shfl_sync(0xffffffffu, upto - mine, src);
       c.b = min(b0 + src, p.B - 1);
-      c.load(p);
-      const long long at = x - start;
-      c.h = (int)(at / c.ntiles);
-      c.t = (int)(at - (long long)c.h * c.ntiles);
+      c.rows = visible_rows(p, c.b);
+      c.h = at / (unsigned)c.rows.n;
+      c.t = at - (unsigned)c.h * c.rows.n;
       return c;
     }
-    before += __shfl_sync(0xffffffffu, upto, 31);
+    at -= __shfl_sync(0xffffffffu, upto, 31);
   }
 }
+
+// The list over n CTAs: the first `rest` take one tile more than the others.
+struct Shares {
+  unsigned each;
+  int rest, n;
+  __device__ __forceinline__ Shares(unsigned total, int n) : n(n) {
+    each = total / (unsigned)n;
+    rest = (int)(total - each * n);
+  }
+  __device__ __forceinline__ unsigned begin(int c) const { return c * each + min(c, rest); }
+  // the CTA that has tile x; a whole warp
+  __device__ __forceinline__ int owner(unsigned x) const {
+    int c = -1;
+    for (int k = lane_id(); k - lane_id() < n; k += 32) c += __popc(__ballot_sync(0xffffffffu, k < n && begin(k) <= x));
+    return c;
+  }
+};
 
 // A part of a pair's result: rows of [D] with their running maximum and sum.
 template <int D>
@@ -137,74 +176,114 @@ struct Part {
   float m[16], l[16];
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_decode_kernel(PagedDecodeParams p) {
-  constexpr int ROWS = kPagedTileBytes / (D * 2);  // rows of a tile
-  constexpr int NT = ROWS / 8;
-  constexpr int RPL = ROWS / 32;                   // rows a lane knows the page of
-  constexpr int CH = D / 8;                        // 16-byte chunks of a row
+// A pair and its tiles' place in the list.
+struct PairSpan {
+  int pair;  // -1: none
+  unsigned start, stop;
+};
+
+// TMA: tiles come as boxes of p.box rows; else row by row with cp.async (pages whose size has no factor of 8).
+template <typename T, int D, bool TMA>
+__global__ void __launch_bounds__(PagedShape<D>::kThreads, 1)
+paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, PagedDecodeParams p) {
+  constexpr int ROWS = kPagedRows, NT = ROWS / 8, CH = D / 8;  // 16-byte chunks of a row
+  constexpr int WARPS = PagedShape<D>::kWarps, THREADS = WARPS * 32, TILE = PagedShape<D>::kTileBytes, RING = PagedShape<D>::kRing;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint8_t* ring = smem + warp * (kPagedStages * 2 * kPagedTileBytes);
-  Part<D>* head_part = reinterpret_cast<Part<D>*>(smem + kPagedWarps * kPagedStages * 2 * kPagedTileBytes) + warp;
+  uint8_t* ring = smem + warp * RING;
+  Part<D>* head_parts = reinterpret_cast<Part<D>*>(smem + WARPS * RING);
   Part<D>* tail_part = reinterpret_cast<Part<D>*>(ring);  // once the ring is empty
-  unsigned* seen_sm = reinterpret_cast<unsigned*>(smem + kPagedWarps * (kPagedStages * 2 * kPagedTileBytes + sizeof(Part<D>))) +
-                      warp * kPagedStages * RPL;
-  // of every warp: pair of its first and of its last part (-1: none), what the CTA joins
-  int* part_pair = reinterpret_cast<int*>(smem + kPagedWarps * (kPagedStages * 2 * kPagedTileBytes + sizeof(Part<D>)) +
-                                          kPagedWarps * kPagedStages * RPL * 4);
-  __shared__ int s_last;
+  __shared__ uint64_t full_bars[WARPS * kPagedStages];
+  __shared__ unsigned seen[WARPS * kPagedStages];
+  __shared__ unsigned before[THREADS];
+  __shared__ unsigned warp_sums[WARPS];
+  __shared__ PairSpan parts[2 * WARPS];  // of each warp's first and of its last part
+  __shared__ PairSpan open[2];           // the CTA's first and last part
+  __shared__ int last_of[2], first_of[2];
+  uint64_t* full = full_bars + warp * kPagedStages;
+  unsigned* seen_sm = seen + warp * kPagedStages;
 
   // ---- this CTA's and this warp's run of tiles ----
-  const long long total = count_tiles<ROWS>(p);
-  const int nc = (int)min((long long)gridDim.x, (total + kPagedWarps - 1) / kPagedWarps);  // CTAs with work
+  const unsigned total = count_tiles<THREADS>(p, before, warp_sums);
+  const int nc = (int)min(gridDim.x, (total + WARPS - 1) / WARPS);  // CTAs with work
   const int cta = blockIdx.x;
   if (cta >= nc) return;
-  const long long c_begin = cta * total / nc, c_end = (cta + 1) * total / nc;
-  const long long begin = c_begin + warp * (c_end - c_begin) / kPagedWarps, end = c_begin + (warp + 1) * (c_end - c_begin) / kPagedWarps;
-  const int count = (int)(end - begin);
-
-  if (lane == 0) part_pair[2 * warp] = part_pair[2 * warp + 1] = -1;
+  const Shares shares(total, nc);
+  const unsigned c_begin = shares.begin(cta), c_end = shares.begin(cta + 1);
+  const int c_count = (int)(c_end - c_begin);
+  const int w_begin = (int)((long long)warp * c_count / WARPS);
+  const int count = (int)((warp + 1ll) * c_count / WARPS) - w_begin;
+  if (smem_u32(smem) & 1023u) {  // the swizzled tiles need a 1024-byte aligned base
+    if (threadIdx.x == 0) p.st.raise(kErrSmemLayout);
+    return;
+  }
+  if (lane == 0) {
+    parts[2 * warp].pair = parts[2 * warp + 1].pair = -1;
+    if (TMA) {
+      for (int s = 0; s < kPagedStages; ++s) mbar_init(full + s, 1);
+      fence_barrier_init();
+    }
+  }
+  if (threadIdx.x < 2) open[threadIdx.x].pair = -1;
+  __syncwarp();
   if (count > 0) {
-    TileCursor<ROWS> cur = find_tile<ROWS>(p, begin), ld = cur;
-    // pages of the tile that is loaded next, a tile ahead of its use
-    int page_id[RPL], slot[RPL];
-    unsigned ok[RPL];
+    TileCursor cur = find_tile<THREADS>(p, before, c_begin + w_begin), ld = cur;
+    // pages of the tile that is loaded next, looked up a tile ahead
+    int page_id, slot;
+    bool in;
     auto look_up = [&](bool more) {
-#pragma unroll
-      for (int r = 0; r < RPL; ++r) {
-        const int u = ld.t * ROWS + r * 32 + lane;
-        const bool in = more && u < ld.rows.n;
-        const int j = u < ld.rows.gap_at ? u : u + ld.rows.gap;
-        const int pg = in ? j / p.page : 0;
-        slot[r] = j - pg * p.page;
-        page_id[r] = in ? __ldg(p.table + (long long)ld.b * p.t_sb + pg) : -1;
-        ok[r] = in;
-      }
+      const int j = ld.row0() + lane;
+      in = more && j < ld.rows.len && (j >= ld.rows.first || j < ld.rows.head);
+      const int pg = in ? j / p.page : 0;
+      slot = j - pg * p.page;
+      page_id = in ? __ldg(p.table + (long long)ld.b * p.t_sb + pg) : -1;
     };
     auto fetch = [&](int i) {  // tile number i of the run into its stage
       const int s = i % kPagedStages;
-      const uint32_t ks = smem_u32(ring + s * 2 * kPagedTileBytes), vs = ks + kPagedTileBytes;
-#pragma unroll
-      for (int r = 0; r < RPL; ++r) {
-        const bool good = ok[r] && (unsigned)page_id[r] < (unsigned)p.num_pages;
-        if (ok[r] && !good) p.st.raise(kErrBadIndex);
-        const unsigned see = __ballot_sync(0xffffffffu, good);
-        if (lane == 0) seen_sm[s * RPL + r] = see;
-        if (!good) page_id[r] = -1;
+      if (ld.t == 0 && lane * 64 < p.G * D) {  // a pair begins: its queries towards this SM
+        const T* qb = static_cast<const T*>(p.q) + (long long)ld.b * p.q_sb + ((long long)ld.h * p.G + lane * 64 / D) * p.q_sh + lane * 64 % D;
+        asm volatile("prefetch.global.L1 [%0];\n" ::"l"(qb));
       }
-      const T* kb = static_cast<const T*>(p.k) + (long long)ld.h * p.k_sh;
-      const T* vb = static_cast<const T*>(p.v) + (long long)ld.h * p.v_sh;
+      uint8_t* ks = ring + s * 2 * TILE;
+      const bool good = in && (unsigned)page_id < (unsigned)p.num_pages;
+      if (in && !good) p.st.raise(kErrBadIndex);
+      const unsigned see = __ballot_sync(0xffffffffu, good);
+      if (lane == 0) seen_sm[s] = see;
+      if (!good) page_id = -1;
+      if constexpr (TMA) {
+        // the lane at the first row of a box issues it, where any of its rows is visible (which says the page)
+        const int at = lane & (p.box - 1);
+        const unsigned mine = see >> (lane - at) & (0xffffffffu >> (32 - p.box));
+        const int src = lane - at + (mine ? __ffs(mine) - 1 : 0);
+        const int pg = __shfl_sync(0xffffffffu, page_id, src), sl = __shfl_sync(0xffffffffu, slot, src) - (src & (p.box - 1));
+        const unsigned boxes = __ballot_sync(0xffffffffu, at == 0 && mine);
+        if (lane == 0) {
+          if (boxes) mbar_expect_tx(full + s, __popc(boxes) * p.box * D * 2 * 2);
+          else mbar_arrive(full + s);
+        }
+        __syncwarp();
+        if (at == 0 && mine) {
 #pragma unroll
-      for (int c = 0; c < ROWS * CH / 32; ++c) {
-        const int flat = c * 32 + lane;
-        const int row = flat / CH, chunk = flat % CH;
-        const int r = c * 32 / CH / 32;  // the same for all lanes
-        const int pg = __shfl_sync(0xffffffffu, page_id[r], row & 31), sl = __shfl_sync(0xffffffffu, slot[r], row & 31);
-        const bool good = pg >= 0;
-        const uint32_t off = swz_addr<ROWS>(0, row, chunk);
-        cp_async16(ks + off, good ? kb + (long long)pg * p.k_sp + (long long)sl * p.k_ss + chunk * 8 : kb, good);
-        cp_async16(vs + off, good ? vb + (long long)pg * p.v_sp + (long long)sl * p.v_ss + chunk * 8 : vb, good);
+          for (int pn = 0; pn < D / 64; ++pn) {
+            uint8_t* dst = ks + pn * ROWS * 128 + lane * 128;
+            tma_load_4d(dst, &tmK, full + s, pn * 64, ld.h, sl, pg);
+            tma_load_4d(dst + TILE, &tmV, full + s, pn * 64, ld.h, sl, pg);
+          }
+        }
+      } else {
+        const uint32_t kb_sm = smem_u32(ks), vb_sm = kb_sm + TILE;
+        const T* kb = static_cast<const T*>(p.k) + (long long)ld.h * p.k_sh;
+        const T* vb = static_cast<const T*>(p.v) + (long long)ld.h * p.v_sh;
+#pragma unroll
+        for (int c = 0; c < ROWS * CH / 32; ++c) {
+          const int flat = c * 32 + lane;
+          const int row = flat / CH, chunk = flat % CH;
+          const int pg = __shfl_sync(0xffffffffu, page_id, row), sl = __shfl_sync(0xffffffffu, slot, row);
+          const bool good = pg >= 0;
+          const uint32_t off = swz_addr<ROWS>(0, row, chunk);
+          cp_async16(kb_sm + off, good ? kb + (long long)pg * p.k_sp + (long long)sl * p.k_ss + chunk * 8 : kb, good);
+          cp_async16(vb_sm + off, good ? vb + (long long)pg * p.v_sp + (long long)sl * p.v_ss + chunk * 8 : vb, good);
+        }
       }
     };
     look_up(true);
@@ -215,21 +294,20 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_decode_kernel(Paged
         ld.next(p);
         look_up(i + 1 < count);
       }
-      cp_async_commit();
+      if (!TMA) cp_async_commit();
     }
 
     uint32_t qf[D / 16][4];
     float o[D / 8][4], m[2], l[2];
-    bool fresh = true;
+    bool fresh = true, first_seg = true;
     int seg_t0 = 0;  // first tile of the present pair in this run
-    bool first_seg = true;
     for (int i = 0; i < count; ++i) {
       if (i + kPagedStages - 1 < count) {
         fetch(i + kPagedStages - 1);
         ld.next(p);
         look_up(i + kPagedStages < count);
       }
-      cp_async_commit();
+      if (!TMA) cp_async_commit();
       if (fresh) {
         const T* qb = static_cast<const T*>(p.q) + (long long)cur.b * p.q_sb + (long long)cur.h * p.G * p.q_sh;
         load_a_frags_global<T, D / 16>(qf, [&](int r) { return r < p.G ? qb + (long long)r * p.q_sh : (const T*)nullptr; });
@@ -240,10 +318,21 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_decode_kernel(Paged
         seg_t0 = cur.t;
         fresh = false;
       }
-      cp_async_wait<kPagedStages - 1>();
-      __syncwarp();
       const int s = i % kPagedStages;
-      const uint32_t ks = smem_u32(ring + s * 2 * kPagedTileBytes), vs = ks + kPagedTileBytes;
+      if (TMA) mbar_wait(full + s, (i / kPagedStages) & 1, p.st);
+      else cp_async_wait<kPagedStages - 1>();
+      __syncwarp();
+      const uint32_t ks = smem_u32(ring + s * 2 * TILE), vs = ks + TILE;
+      const unsigned see = seen_sm[s];
+      if (TMA && see != 0xffffffffu) {
+        // rows that are not visible may hold anything, and 0 times that is not 0 where it is not finite
+        if (!(see >> lane & 1u))
+#pragma unroll
+          for (int c = 0; c < CH; ++c)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(swz_addr<ROWS>(vs, lane, c)), "r"(0) : "memory");
+        fence_proxy_async();  // TMA writes there again
+        __syncwarp();
+      }
       float x[NT][4];
 #pragma unroll
       for (int j = 0; j < NT; ++j) x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.f;
@@ -253,10 +342,10 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_decode_kernel(Paged
       float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const unsigned see = seen_sm[s * RPL + j / 4] >> ((j & 3) * 8 + c0);
+        const unsigned bits = see >> (j * 8 + c0);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[j][e] = (see >> (e & 1)) & 1u ? x[j][e] * p.scale2 : -INFINITY;
+          x[j][e] = (bits >> (e & 1)) & 1u ? x[j][e] * p.scale2 : -INFINITY;
           mx[e >> 1] = fmaxf(mx[e >> 1], x[j][e]);
         }
       }
@@ -266,12 +355,12 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_decode_kernel(Paged
         for (int half = 0; half < 2; ++half) {
           const int g = (lane >> 2) + half * 8;
           if (g < p.G) {
-            float* dst = p.logits + (pair * p.G + g) * p.cap + cur.t * ROWS;
+            const int at = cur.row0() + c0;
+            float* dst = p.logits + (pair * p.G + g) * p.cap + at;
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-              const int u = cur.t * ROWS + j * 8 + c0;
-              if (u < cur.rows.n) dst[j * 8 + c0] = x[j][2 * half];
-              if (u + 1 < cur.rows.n) dst[j * 8 + c0 + 1] = x[j][2 * half + 1];
+              if (at + j * 8 < p.cap) dst[j * 8] = x[j][2 * half];
+              if (at + j * 8 + 1 < p.cap) dst[j * 8 + 1] = x[j][2 * half + 1];
             }
           }
         }
@@ -292,14 +381,16 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_decode_kernel(Paged
           x[j][e] = fast_exp2(x[j][e] - base[e >> 1]);
           sum[e >> 1] += x[j][e];
         }
-      l[0] = l[0] * corr[0] + quad_sum(sum[0]);
-      l[1] = l[1] * corr[1] + quad_sum(sum[1]);
+      l[0] = l[0] * corr[0] + sum[0];  // of this lane's columns
+      l[1] = l[1] * corr[1] + sum[1];
+      if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
 #pragma unroll
-      for (int j = 0; j < D / 8; ++j) {
-        o[j][0] *= corr[0];
-        o[j][1] *= corr[0];
-        o[j][2] *= corr[1];
-        o[j][3] *= corr[1];
+        for (int j = 0; j < D / 8; ++j) {
+          o[j][0] *= corr[0];
+          o[j][1] *= corr[0];
+          o[j][2] *= corr[1];
+          o[j][3] *= corr[1];
+        }
       }
       uint32_t hi[NT / 2][4], lo[NT / 2][4];
 #pragma unroll
@@ -328,8 +419,10 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_decode_kernel(Paged
       }
       __syncwarp();  // the stage has been read
       // ---- the end of the pair or of the run ----
-      const bool pair_ends = cur.t + 1 == cur.ntiles;
+      const bool pair_ends = cur.t + 1 == cur.rows.n;
       if (pair_ends || i + 1 == count) {
+        l[0] = quad_sum(l[0]);
+        l[1] = quad_sum(l[1]);
         const int pair = cur.b * p.Hkv + cur.h;
         const int r0 = lane >> 2;
         if (pair_ends && seg_t0 == 0) {
@@ -347,12 +440,8 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_decode_kernel(Paged
             }
           }
         } else {
-          const bool tail = !first_seg;  // the run's last part, and its ring is empty
-          if (tail) {
-            cp_async_wait<0>();
-            __syncwarp();
-          }
-          Part<D>* dst = tail ? tail_part : head_part;
+          const bool tail = !first_seg;  // the run's last part: nothing is on its way into the ring
+          Part<D>* dst = tail ? tail_part : head_parts + warp;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int g = r0 + half * 8;
@@ -363,118 +452,171 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_decode_kernel(Paged
               dst->l[g] = l[half];
             }
           }
-          if (lane == 0) part_pair[2 * warp + tail] = pair;
+          if (lane == 0) {
+            const unsigned start = c_begin + w_begin + i - cur.t;
+            parts[2 * warp + tail] = PairSpan{pair, start, start + cur.rows.n};
+          }
         }
         first_seg = false;
         fresh = true;
       }
       cur.next(p);
     }
-    cp_async_wait<0>();
+    if (!TMA) cp_async_wait<0>();
   }
   __syncthreads();
 
-  // ---- join the parts: first the CTA's, in order, then those of other CTAs ----
-  auto part_at = [&](int i) -> Part<D>* {
-    return (i & 1) ? reinterpret_cast<Part<D>*>(smem + (i >> 1) * (kPagedStages * 2 * kPagedTileBytes))
-                   : reinterpret_cast<Part<D>*>(smem + kPagedWarps * kPagedStages * 2 * kPagedTileBytes) + (i >> 1);
-  };
-  auto write_row = [&](int pair, int g, int col, float val, float mm, float ll) {
-    const int b = pair / p.Hkv, h = pair - b * p.Hkv;
-    T* ob = static_cast<T*>(p.o) + (long long)b * p.o_sb + (long long)(h * p.G + g) * p.o_sh;
-    ob[col] = DT<T>::from_float(ll > 0.f ? val / ll : 0.f);
-    if (p.lse && col == 0) p.lse[(long long)pair * p.G + g] = ll > 0.f ? mm + log2f(ll) : -INFINITY;
-  };
-  constexpr int PART_FLOATS = 16 * (D + 2);
-  for (int i = 0; i < 2 * kPagedWarps;) {
-    const int pair = part_pair[i];
-    if (pair < 0) {
-      ++i;
-      continue;
-    }
-    int e = i + 1;  // parts [i, e) of the pair
-    while (e < 2 * kPagedWarps && (part_pair[e] == pair || part_pair[e] < 0)) ++e;
-    // where the pair's tiles lie in the list
-    TileCursor<ROWS> at;
-    long long start = 0;
-    {
-      const int b = pair / p.Hkv;
-      for (int x = lane; x < b; x += 32) start += tiles_of<ROWS>(p, x);
+  // ---- join the CTA's parts of each pair in order: a warp a pair, or a part of its rows where there are fewer pairs than warps ----
+  constexpr int PART_FLOATS = 16 * (D + 2), EPL = D / 32, RY = 16 / WARPS;  // columns of a lane, rows at a time
+  typedef typename std::conditional<EPL == 4, float4, float2>::type Cols;
+  auto fma_cols = [](float (&a)[EPL], float w, Cols x) {
+    const float* e = reinterpret_cast<const float*>(&x);
 #pragma unroll
-      for (int s = 16; s; s >>= 1) start += __shfl_xor_sync(0xffffffffu, start, s);
-      at.b = b;
-      at.load(p);
-      start = start * p.Hkv + (long long)(pair - b * p.Hkv) * at.ntiles;
-    }
-    const long long stop = start + at.ntiles;
-    const bool whole = start >= c_begin && stop <= c_end;
-    float* mine = p.part + ((long long)cta * 2 + (start < c_begin ? 0 : 1)) * PART_FLOATS;
-    for (int f = threadIdx.x; f < p.G * D; f += kPagedWarps * 32) {
-      const int g = f / D, col = f % D;
-      float mm = -INFINITY;
-      for (int x = i; x < e; ++x)
-        if (part_pair[x] == pair) mm = fmaxf(mm, part_at(x)->m[g]);
-      const float base = mm == -INFINITY ? 0.f : mm;
-      float val = 0.f, ll = 0.f;
-      for (int x = i; x < e; ++x)
-        if (part_pair[x] == pair) {
-          const float w = fast_exp2(part_at(x)->m[g] - base);
-          val += w * part_at(x)->o[g][col];
-          ll += w * part_at(x)->l[g];
+    for (int c = 0; c < EPL; ++c) a[c] = fmaf(w, e[c], a[c]);
+  };
+  auto write_row = [&](int pair, int g, const float (&val)[EPL], float mm, float ll) {
+    const int b = pair / p.Hkv, h = pair - b * p.Hkv;
+    const float inv = ll > 0.f ? 1.f / ll : 0.f;
+    uint32_t* row = reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + (long long)b * p.o_sb + (long long)(h * p.G + g) * p.o_sh + lane * EPL);
+#pragma unroll
+    for (int c = 0; c < EPL; c += 2) row[c / 2] = DT<T>::pack(val[c] * inv, val[c + 1] * inv);
+    if (p.lse && lane == 0) p.lse[(long long)pair * p.G + g] = ll > 0.f ? mm + log2f(ll) : -INFINITY;
+  };
+  {
+    auto part_at = [&](int i) { return (i & 1) ? reinterpret_cast<const Part<D>*>(smem + (i >> 1) * RING) : head_parts + (i >> 1); };
+    const PairSpan mine = lane < 2 * WARPS ? parts[lane] : PairSpan{-1, 0, 0};
+    const unsigned present = __ballot_sync(0xffffffffu, mine.pair >= 0), below = present & ((1u << lane) - 1u);
+    const int prev = __shfl_sync(0xffffffffu, mine.pair, below ? 31 - __clz(below) : 0);
+    const unsigned starts = __ballot_sync(0xffffffffu, mine.pair >= 0 && (!below || prev != mine.pair));
+    const int pairs = __popc(starts);
+    int slices = 1;
+    if (pairs > 0)
+      while (2 * slices * pairs <= WARPS) slices *= 2;
+    const int per = (p.G + slices - 1) / slices;  // rows of a slice
+    for (int item = warp; item < pairs * slices; item += WARPS) {
+      unsigned from = starts;
+      for (int k = item / slices; k; --k) from &= from - 1;
+      const int a = __ffs(from) - 1;
+      const unsigned later = from & (from - 1);
+      const unsigned members = present & (0xffffffffu << a) & (later ? (later & -later) - 1u : 0xffffffffu);
+      const PairSpan w{__shfl_sync(0xffffffffu, mine.pair, a), __shfl_sync(0xffffffffu, mine.start, a), __shfl_sync(0xffffffffu, mine.stop, a)};
+      const bool whole = w.start >= c_begin && w.stop <= c_end;
+      const int which = w.start < c_begin ? 0 : 1, slice = item % slices;
+      float* out = p.part + ((long long)cta * 2 + which) * PART_FLOATS;
+      // factors and sums of RY rows at a time, a lane a part and row; then their columns
+      const int x = lane % (2 * WARPS);
+      const bool has = members >> x & 1u;
+      const Part<D>* own = part_at(has ? x : a);
+      for (int g0 = slice * per; g0 < min(p.G, (slice + 1) * per); g0 += RY) {
+        const int g = min(g0 + lane / (2 * WARPS), 15);
+        const float pm = has ? own->m[g] : -INFINITY, pl = has ? own->l[g] : 0.f;
+        float mm = pm;
+#pragma unroll
+        for (int s = WARPS; s; s >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, s));
+        const float f = fast_exp2(pm - (mm == -INFINITY ? 0.f : mm));
+        float ll = f * pl;
+#pragma unroll
+        for (int s = WARPS; s; s >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, s);
+        alignas(16) float val[RY][EPL] = {};
+        for (unsigned rem = members; rem; rem &= rem - 1) {
+          const int y = __ffs(rem) - 1;
+          const float* src = &part_at(y)->o[0][lane * EPL];
+#pragma unroll
+          for (int r = 0; r < RY; ++r)
+            fma_cols(val[r], __shfl_sync(0xffffffffu, f, r * 2 * WARPS + y), *reinterpret_cast<const Cols*>(src + min(g0 + r, 15) * D));
         }
-      if (whole) {
-        write_row(pair, g, col, val, mm, ll);
-      } else {
-        mine[g * D + col] = val;
-        if (col == 0) {
-          mine[16 * D + g] = mm;
-          mine[16 * D + 16 + g] = ll;
-        }
-      }
-    }
-    if (!whole) {
-      const int first = (int)(((start + 1) * nc - 1) / total), last = (int)((stop * nc - 1) / total);  // CTAs that hold some of it
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) s_last = atomicInc(p.ctrl + first, (unsigned)(last - first)) == (unsigned)(last - first);
-      __syncthreads();
-      if (s_last) {
-        __threadfence();
-        for (int f = threadIdx.x; f < p.G * D; f += kPagedWarps * 32) {
-          const int g = f / D, col = f % D;
-          auto of = [&](int c) { return p.part + ((long long)c * 2 + (c == first ? 1 : 0)) * PART_FLOATS; };
-          float mm = -INFINITY;
-          for (int c = first; c <= last; ++c) mm = fmaxf(mm, __ldcg(of(c) + 16 * D + g));
-          const float base = mm == -INFINITY ? 0.f : mm;
-          float val = 0.f, ll = 0.f;
-          for (int c = first; c <= last; ++c) {
-            const float w = fast_exp2(__ldcg(of(c) + 16 * D + g) - base);
-            val += w * __ldcg(of(c) + g * D + col);
-            ll += w * __ldcg(of(c) + 16 * D + 16 + g);
+#pragma unroll
+        for (int r = 0; r < RY; ++r) {
+          const float m1 = __shfl_sync(0xffffffffu, mm, r * 2 * WARPS), l1 = __shfl_sync(0xffffffffu, ll, r * 2 * WARPS);
+          if (g0 + r >= min(p.G, (slice + 1) * per)) continue;
+          if (whole) {
+            write_row(w.pair, g0 + r, val[r], m1, l1);
+          } else {
+            *reinterpret_cast<Cols*>(out + (g0 + r) * D + lane * EPL) = *reinterpret_cast<const Cols*>(val[r]);
+            if (lane == 0) *reinterpret_cast<float2*>(out + 16 * D + 2 * (g0 + r)) = make_float2(m1, l1);
           }
-          write_row(pair, g, col, val, mm, ll);
         }
       }
-      __syncthreads();
+      if (!whole && slice == 0 && lane == 0) open[which] = w;
     }
-    i = e;
+  }
+  __syncthreads();
+
+  // ---- what other CTAs have parts of: the last of them joins, 16 / WARPS rows a warp ----
+  if (warp < 2) {
+    const PairSpan w = open[warp];
+    if (w.pair >= 0) {
+      const int first = shares.owner(w.start), n = shares.owner(w.stop - 1) - first + 1;
+      if (lane == 0) {  // (one thread's fences: the CTA's barriers stand on either side)
+        __threadfence();
+        last_of[warp] = atomicInc(p.ctrl + first, (unsigned)(n - 1)) == (unsigned)(n - 1) ? n : 0;
+        first_of[warp] = first;
+        __threadfence();
+      }
+    } else if (lane == 0) {
+      last_of[warp] = 0;
+    }
+  }
+  __syncthreads();
+  for (int x = 0; x < 2; ++x) {
+    const int n = last_of[x];
+    if (n == 0) continue;
+    const int pair = open[x].pair, first = first_of[x];
+    auto of = [&](int c) { return p.part + ((long long)(first + c) * 2 + (c == 0 ? 1 : 0)) * PART_FLOATS; };
+    // four parts of RY rows on their way at a time
+    float mm[RY], ll[RY], val[RY][EPL] = {};
+#pragma unroll
+    for (int r = 0; r < RY; ++r) mm[r] = -INFINITY, ll[r] = 0.f;
+    for (int c0 = 0; c0 < n; c0 += 4) {
+      float2 ml[4][RY];
+      Cols o[4][RY];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float* src = of(min(c0 + c, n - 1));
+#pragma unroll
+        for (int r = 0; r < RY; ++r) {
+          const int g = min(warp * RY + r, p.G - 1);
+          ml[c][r] = __ldcg(reinterpret_cast<const float2*>(src + 16 * D + 2 * g));
+          o[c][r] = __ldcg(reinterpret_cast<const Cols*>(src + g * D + lane * EPL));
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < RY; ++r) {
+        float now = mm[r];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) now = fmaxf(now, ml[c][r].x);
+        const float base = now == -INFINITY ? 0.f : now, old = fast_exp2(mm[r] - base);
+        mm[r] = now;
+        ll[r] *= old;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) val[r][e] *= old;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float f = c0 + c < n ? fast_exp2(ml[c][r].x - base) : 0.f;
+          ll[r] = fmaf(f, ml[c][r].y, ll[r]);
+          fma_cols(val[r], f, o[c][r]);
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < RY; ++r)
+      if (warp * RY + r < p.G) write_row(pair, warp * RY + r, val[r], mm[r], ll[r]);
   }
 }
 
 // weights[b][h][j] += sum over the G heads of 2^(x_j - lse), row by row of the logits the attention kernel left.
 __global__ void __launch_bounds__(256) paged_weights_kernel(PagedDecodeParams p, float* weights, long long w_sb, long long w_sh) {
   const int b = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv;
-  const Rows rows = visible_rows(__ldg(p.seqlens + b), p.window, p.sinks, p.cap);
-  const int u = blockIdx.y * 256 + threadIdx.x;
-  if (u >= rows.n) return;
-  const float* x = p.logits + (long long)blockIdx.x * p.G * p.cap + u;
+  const Rows rows = visible_rows(p, b);
+  const int j = blockIdx.y * 256 + threadIdx.x;
+  if (j >= rows.len || (j >= rows.head && j < rows.first)) return;
+  const float* x = p.logits + (long long)blockIdx.x * p.G * p.cap + j;
   const float* lse = p.lse + (long long)blockIdx.x * p.G;
   float sum = 0.f;
   for (int g = 0; g < p.G; ++g) {
     const float ls = __ldg(lse + g);
     sum += ls == -INFINITY ? 0.f : fast_exp2(__ldg(x + (long long)g * p.cap) - ls);
   }
-  const int j = u < rows.gap_at ? u : u + rows.gap;
   weights[b * w_sb + h * w_sh + j] += sum;
 }
 
@@ -484,18 +626,29 @@ static long long paged_part_floats(int D) { return (long long)num_sms() * 2 * 16
 
 template <typename T, int D>
 static int launch_paged_decode(PagedDecodeParams p, float* weights, long long w_sb, long long w_sh, cudaStream_t stream) {
-  constexpr int ROWS = kPagedTileBytes / (D * 2);
-  const size_t smem = kPagedWarps * (kPagedStages * 2 * kPagedTileBytes + sizeof(Part<D>)) + kPagedWarps * kPagedStages * (ROWS / 32) * 4 +
-                      2 * kPagedWarps * sizeof(int);
-  auto kern = paged_decode_kernel<T, D>;
+  constexpr int WARPS = PagedShape<D>::kWarps;
+  const size_t smem = WARPS * (PagedShape<D>::kRing + sizeof(Part<D>));
+  // the largest power of two that divides a page, at most 32
+  p.box = std::min(32, p.page & -p.page);
+  const bool tma = p.box >= 8;
+  CUtensorMap tmK{}, tmV{};
+  if (tma) {
+    int rc = make_tmap_4d(&tmK, DT<T>::kTmapType, p.k, D, p.Hkv, p.page, p.num_pages, p.k_sh, p.k_ss, p.k_sp, 64, p.box, 1);
+    if (!rc) rc = make_tmap_4d(&tmV, DT<T>::kTmapType, p.v, D, p.Hkv, p.page, p.num_pages, p.v_sh, p.v_ss, p.v_sp, 64, p.box, 1);
+    if (rc) return rc;
+  }
+  auto kern = tma ? paged_decode_kernel<T, D, true> : paged_decode_kernel<T, D, false>;
   cudaError_t e = allow_smem(kern, smem);
   if (e != cudaSuccess) return cuda_rc(e);
-  const long long most = (long long)p.B * p.Hkv * std::max(1, (p.cap + ROWS - 1) / ROWS);
-  const int grid = (int)std::min<long long>(num_sms(), (most + kPagedWarps - 1) / kPagedWarps);
-  { LaunchScope ls_("paged_decode", stream); kern<<<grid, kPagedWarps * 32, smem, stream>>>(p); }
+  const long long most = (long long)p.B * p.Hkv * ((p.cap + kPagedRows - 1) / kPagedRows);
+  const int grid = (int)std::min<long long>(num_sms(), (most + WARPS - 1) / WARPS);
+  { LaunchScope ls_("paged_decode", stream); kern<<<grid, WARPS * 32, smem, stream>>>(tmK, tmV, p); }
   e = cudaGetLastError();
   if (e != cudaSuccess || !weights) return cuda_rc(e);
-  { LaunchScope ls_("paged_weights", stream); paged_weights_kernel<<<dim3(p.B * p.Hkv, (p.cap + 255) / 256), 256, 0, stream>>>(p, weights, w_sb, w_sh); }
+  {
+    LaunchScope ls_("paged_weights", stream);
+    paged_weights_kernel<<<dim3(p.B * p.Hkv, (p.cap + 255) / 256), 256, 0, stream>>>(p, weights, w_sb, w_sh);
+  }
   return cuda_rc(cudaGetLastError());
 }
 
@@ -516,7 +669,8 @@ extern "C" int nsa_paged_attn_decode(const void* q, const void* k_pages, const v
   if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads) return kInvalid;
   if (num_pages <= 0 || page_size <= 0 || max_pages <= 0 || num_sinks < 0) return kInvalid;
   const long long cap = (long long)page_size * max_pages;
-  if (cap > (1ll << 30) || (long long)batch * num_kv_heads > (1ll << 30)) return kUnsupported;
+  // tiles are counted in 32 bits
+  if (cap > (1ll << 30) || (long long)batch * num_kv_heads > (1ll << 30) || (double)batch * num_kv_heads * (cap + 31) >= 0x1p36) return kUnsupported;
   if (num_q_heads / num_kv_heads > 16) return kUnsupported;
   if (weights && cap > 65535 * 256) return kUnsupported;
   // strides: q_b q_h  k_page k_slot k_h  v_page v_slot v_h  o_b o_h  table_b  weights_b weights_h

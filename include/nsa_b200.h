@@ -226,13 +226,15 @@ int nsa_window_attn_bwd(const void* q, const void* k, const void* v, const void*
 
 /* Sliding window with sinks: query t of a sequence sees key j <= t iff t - j <= window_left or j < num_sinks.  No counterpart in the
  * reference.  Tensors, strides and lse convention as nsa_window_attn_fwd / nsa_window_attn_bwd, head_dim 64 or 128; no bound on the lengths
- * is needed.  Output, dq, dk and dv of rows behind the last sequence are zero.  Workspace: nsa_sink_window_attn_bwd_workspace bytes. */
-int nsa_sink_window_attn_fwd(const void* q, const void* k, const void* v, const int* cu_seqlens, void* o, float* lse, int total_len,
-                             int batch, int num_q_heads, int num_kv_heads, int head_dim, int window_left, int num_sinks,
+ * is needed.  Output, dq, dk and dv of rows behind the last sequence are zero.  o_rest: NULL, or total_len * num_q_heads * d 16-bit
+ * elements, 16-byte aligned, that the forward fills for the backward in an order of its own with what the rounding of o took away: with it
+ * sum_d o dO is exact to 2^-17 (2^-22), which rows that look at few keys need.  Workspace: nsa_sink_window_attn_bwd_workspace bytes. */
+int nsa_sink_window_attn_fwd(const void* q, const void* k, const void* v, const int* cu_seqlens, void* o, void* o_rest, float* lse,
+                             int total_len, int batch, int num_q_heads, int num_kv_heads, int head_dim, int window_left, int num_sinks,
                              const long long* strides, float sm_scale, int dtype, void* stream);
 long long nsa_sink_window_attn_bwd_workspace(int total_len, int num_q_heads, int num_kv_heads, int head_dim);
-int nsa_sink_window_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse,
-                             const int* cu_seqlens, void* dq, void* dk, void* dv, void* workspace, long long workspace_bytes,
+int nsa_sink_window_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* dout,
+                             const float* lse, const int* cu_seqlens, void* dq, void* dk, void* dv, void* workspace, long long workspace_bytes,
                              int total_len, int batch, int num_q_heads, int num_kv_heads, int head_dim, int window_left, int num_sinks,
                              const long long* strides, float sm_scale, int dtype, void* stream);
 

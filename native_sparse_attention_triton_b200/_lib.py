@@ -36,8 +36,8 @@ _SIGNATURES = {
     "nsa_pool_compress_fwd": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _L, _L, _I, _P],
     "nsa_varlen_attn_bwd": [_P] * 12 + [_L] + [_I] * 11 + [_P, _F, _I, _P],
     "nsa_window_attn_bwd": [_P] * 11 + [_L] + [_I] * 7 + [_P, _F, _I, _P],
-    "nsa_sink_window_attn_fwd": [_P] * 6 + [_I] * 7 + [_P, _F, _I, _P],
-    "nsa_sink_window_attn_bwd": [_P] * 11 + [_L] + [_I] * 7 + [_P, _F, _I, _P],
+    "nsa_sink_window_attn_fwd": [_P] * 7 + [_I] * 7 + [_P, _F, _I, _P],
+    "nsa_sink_window_attn_bwd": [_P] * 12 + [_L] + [_I] * 7 + [_P, _F, _I, _P],
     "nsa_paged_kv_append": [_P] * 8 + [_I] * 7 + [_P, _P],
     "nsa_paged_attn_decode": [_P] * 8 + [_L] + [_I] * 9 + [_P, _F, _I, _P],
     "nsa_paged_kv_evict": [_P] * 9 + [_I] * 10 + [_P, _P],

@@ -861,7 +861,7 @@ __global__ void __launch_bounds__(256) sink_finish_kernel(DkdvParams p, const __
 }
 
 template <typename T, int D>
-static int run_sink_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, const int* cu, void* dq,
+static int run_sink_bwd(const void* q, const void* k, const void* v, const void* o, const void* rest, const void* dout, const float* lse, const int* cu, void* dq,
                         void* dk, void* dv, void* ws, int total, int batch, int Hq, int Hkv, int left, int sinks, const long long* S, float sm_scale,
                         cudaStream_t stream) {
   const int G = Hq / Hkv;
@@ -880,11 +880,12 @@ static int run_sink_bwd(const void* q, const void* k, const void* v, const void*
   p.B = batch; p.Hq = Hq; p.Hkv = Hkv; p.G = G;
   p.logG = 0;
   while ((1 << p.logG) < G) ++p.logG;
-  p.window = 1; p.stride = 1; p.causal = 1; p.left = left; p.sinks = sinks;
+  p.window = 1; p.stride = 1; p.causal = 1; p.left = left; p.sinks = sinks; p.rest = static_cast<const uint4*>(rest);
   p.scale2 = sm_scale * kLog2e; p.sm_scale = sm_scale;
   p.st.word = status_word();
   const int dt = DT<T>::kTmapType == CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 ? NSA_DTYPE_BF16 : NSA_DTYPE_FP16;
-  int rc = dense_dq_tc(k, v, S[2], S[3], S[4], S[5], total, total, total, D, dt, p, stream);
+  const long long ds[8] = {S[0], S[1], S[2], S[3], S[4], S[5], S[8], S[9]};
+  int rc = sink_dq_tc(k, v, ds, total, D, dt, p, stream);
   if (rc) return rc;
   DkdvParams d;
   d.ld = ld; d.dk32 = dk32; d.dv32 = dv32; d.cu_q = cu; d.cu_k = cu;
@@ -896,11 +897,10 @@ static int run_sink_bwd(const void* q, const void* k, const void* v, const void*
   d.key_slots = (int)row_tile_slots(total, batch, 7);
   d.sink_log = 13 - p.logG;  // 64 row tiles
   while (d.sink_log > 9 - p.logG && row_tile_slots(total, batch, d.sink_log) * Hkv < 148) --d.sink_log;
-  const long long ds[8] = {S[0], S[1], S[2], S[3], S[4], S[5], S[8], S[9]};
   rc = launch_dense_dkdv_tc<T, D>(q, dout, k, v, ds, total, total, (int)std::min<long long>(total, (long long)left + 128), 0, batch, d, stream);
   if (rc) return rc;
   SinkMaps maps;
-  rc = make_sink_maps(maps, DT<T>::kTmapType, q, k, v, dout, ds, D, Hkv, total, sinks);
+  rc = make_sink_maps(maps, DT<T>::kTmapType, q, k, v, dout, ds, D, Hkv, total, sinks, 128);
   if (rc) return rc;
   LaunchScope ls_("sink_finish", stream);
   sink_finish_kernel<T, D><<<(unsigned)(((long long)total * Hkv + 7) / 8), 256, 0, stream>>>(d, maps, dk, dv, S[12], S[13], S[14], S[15], total);
@@ -1115,8 +1115,8 @@ extern "C" long long nsa_sink_window_attn_bwd_workspace(int total_len, int num_q
   return (long long)nsa::dense_ws_bytes(total_len, total_len, num_q_heads, num_kv_heads, head_dim);
 }
 
-extern "C" int nsa_sink_window_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse,
-                                        const int* cu_seqlens, void* dq, void* dk, void* dv, void* workspace, long long workspace_bytes,
+extern "C" int nsa_sink_window_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* dout,
+                                        const float* lse, const int* cu_seqlens, void* dq, void* dk, void* dv, void* workspace, long long workspace_bytes,
                                         int total_len, int batch, int num_q_heads, int num_kv_heads, int head_dim, int window_left,
                                         int num_sinks, const long long* strides, float sm_scale, int dtype, void* stream) {
   using namespace nsa;
@@ -1128,8 +1128,9 @@ extern "C" int nsa_sink_window_attn_bwd(const void* q, const void* k, const void
     if (strides[i] % 8) return kInvalid;
   for (const void* rows : {q, k, v, o, dout, (const void*)dq, (const void*)dk, (const void*)dv})  // read and written 16 bytes at a time
     if (!aligned16(rows)) return kInvalid;
+  if (!aligned16(o_rest)) return kInvalid;
   if (workspace_bytes < nsa_sink_window_attn_bwd_workspace(total_len, num_q_heads, num_kv_heads, head_dim)) return kWorkspace;
-  return NSA_DISPATCH_T_D(dtype, head_dim, run_sink_bwd, q, k, v, o, dout, lse, cu_seqlens, dq, dk, dv, workspace, total_len, batch, num_q_heads,
+  return NSA_DISPATCH_T_D(dtype, head_dim, run_sink_bwd, q, k, v, o, o_rest, dout, lse, cu_seqlens, dq, dk, dv, workspace, total_len, batch, num_q_heads,
                           num_kv_heads, std::min(window_left, total_len), std::min(num_sinks, total_len), strides, sm_scale,
                           static_cast<cudaStream_t>(stream));
 }

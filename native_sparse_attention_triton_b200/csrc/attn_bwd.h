@@ -70,16 +70,20 @@ struct DenseBwdParams {
   Status st;
   int sinks = -1;  // >= 0: sliding window with sinks (... or key < sinks)
   int rows = 0;    // of dq
+  const uint4* rest = nullptr;  // what the rounding of o took away (rest_chunk in sink_keys.cuh), or nullptr
 };
 
 struct SinkMaps;
-// strides S: q_n q_h k_n k_h v_n v_h do_n do_h (the last two where dout is given)
+// strides S: q_n q_h k_n k_h v_n v_h do_n do_h (the last two where dout is given); tile: rows of a key tile
 int make_sink_maps(SinkMaps& m, CUtensorMapDataType dt, const void* q, const void* k, const void* v, const void* dout, const long long* S, int D,
-                   int Hkv, int Nk, int sinks);
+                   int Hkv, int Nk, int sinks, int tile);
 
 // tcgen05 implementation of the dense dQ pass (dense_dq_tc.cu).  k/v strides in elements.
 int dense_dq_tc(const void* k, const void* v, long long k_sn, long long k_sh, long long v_sn, long long v_sh, int total_q,
                 int total_k, int max_seqlen_q, int head_dim, int dtype, DenseBwdParams p, cudaStream_t stream);
+
+// dQ pass of the sliding window with sinks (sink_dq_tc.cu); strides: q_n q_h k_n k_h v_n v_h do_n do_h
+int sink_dq_tc(const void* k, const void* v, const long long* strides, int total, int head_dim, int dtype, DenseBwdParams p, cudaStream_t stream);
 
 // tcgen05 dK/dV pass of the top-k sparse attention (sparse_dkdv_tc.cu); head_dim 64 and 128, group size 4, 8 or 16.
 // strides: q_n q_h k_n k_h v_n v_h do_n do_h (elements); grid = (work items, 64-key tiles per block).

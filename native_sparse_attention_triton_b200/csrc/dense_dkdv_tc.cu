@@ -278,7 +278,13 @@ dense_dkdv_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       mbar_wait(s_full, i & 1, p.st);
       tc_fence_after_sync();
       float pf[64];
-      {
+      // a row tile that no key of the warp is seen by: at the edges of a window that is every other one
+      const bool none = SINKS && __all_sync(0xffffffffu, span == 0u);
+      if (none) {
+        const uint32_t zero[32] = {};
+        tmem_st32(lane_base + 256 + half * 64, zero);
+        tmem_st_wait();
+      } else {
         uint32_t su[2][32];
         tmem_ld32(lane_base + 256 + half * 64, su[0]);
         tmem_ld32(lane_base + 256 + half * 64 + 32, su[1]);
@@ -296,7 +302,11 @@ dense_dkdv_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 
       mbar_wait(dp_full, i & 1, p.st);
       tc_fence_after_sync();
-      {
+      if (none) {
+        const uint32_t zero[32] = {};
+        tmem_st32(lane_base + 384 + half * 64, zero);
+        tmem_st_wait();
+      } else {
         uint32_t du[2][32];
         tmem_ld32(lane_base + 384 + half * 64, du[0]);
         tmem_ld32(lane_base + 384 + half * 64 + 32, du[1]);

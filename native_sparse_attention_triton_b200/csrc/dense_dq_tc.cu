@@ -20,10 +20,7 @@
 #include "attn_tile.cuh"
 #include "dispatch.h"
 #include "host_util.h"
-#include "sink_exact.cuh"
-#include "sink_keys.cuh"
 #include "tc5.cuh"
-#include "work_steal.cuh"
 
 namespace nsa {
 
@@ -32,13 +29,11 @@ constexpr int kDqKStages = 3;
 constexpr int kDqVStages = 2;
 }
 
-// SINKS: a sliding window with sinks; the CTA's key tiles are those of its rows' list of keys (sink_keys.cuh), and the sequence of its row
-// tile is searched for.
-template <typename T, int D, bool SINKS>
+template <typename T, int D>
 __global__ void __launch_bounds__(320, 1)
 dense_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
                    const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                   const __grid_constant__ CUtensorMap tmDQ, DenseBwdParams p, const __grid_constant__ TileMaps<SINKS> split) {
+                   const __grid_constant__ CUtensorMap tmDQ, DenseBwdParams p) {
   constexpr int KT = 128;
   constexpr int PANELS = D / 64;
   constexpr int PANEL_BYTES = 128 * 128;
@@ -70,20 +65,13 @@ dense_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     if (threadIdx.x == 0) p.st.raise(kErrSmemLayout);
     return;
   }
+  const int b = blockIdx.y, h = blockIdx.z;
+  const int qs = __ldg(p.cu_q + b), Lq = __ldg(p.cu_q + b + 1) - qs;
+  const int ksq = __ldg(p.cu_k + b), Lk = __ldg(p.cu_k + b + 1) - ksq;
   const int QT = 128 >> p.logG;
-  int b = blockIdx.y, qs, Lq, qt = gridDim.x - 1 - blockIdx.x;
-  const int h = blockIdx.z;
-  if constexpr (SINKS) {
-    if (threadIdx.x < 32)
-      zero_rows_behind<T, D>(p.dq, p.dq_sn, p.dq_sh, __ldg(p.cu_q + p.B), p.rows, blockIdx.x, gridDim.x, h * p.G, p.G);
-    if (!find_row_tile(p.cu_q, p.B, 7 - p.logG, gridDim.x - 1 - blockIdx.x, b, qs, Lq, qt)) return;
-  } else {
-    qs = __ldg(p.cu_q + b);
-    Lq = __ldg(p.cu_q + b + 1) - qs;
-  }
+  const int qt = gridDim.x - 1 - blockIdx.x;
   const int q0 = qt * QT;
   if (q0 >= Lq) return;
-  const int ksq = __ldg(p.cu_k + b), Lk = __ldg(p.cu_k + b + 1) - ksq;
   auto visible = [&](int t) {
     if (!p.causal) return Lk;
     return t < p.window - 1 ? 0 : min(Lk, (t - p.window + 1) / p.stride + 1);
@@ -91,9 +79,7 @@ dense_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   const int t_hi = min(q0 + QT, Lq) - 1;
   // with a sliding window the first key tiles are invisible to every row of the CTA: start at tile kt0
   const int kt0 = p.left >= 0 ? max(0, q0 - p.left) / KT : 0;
-  const int shift = SINKS ? sink_shift(q0, p.left, sink_room(p.sinks)) : 0;
-  const int columns = t_hi + 1 - shift;  // of the list of keys
-  const int ntiles = SINKS ? (columns + KT - 1) / KT : max(0, (visible(t_hi) + KT - 1) / KT - kt0);
+  const int ntiles = max(0, (visible(t_hi) + KT - 1) / KT - kt0);
 
   if (threadIdx.x == 0) {
     mbar_init(qdo_full, 1);
@@ -139,13 +125,9 @@ dense_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         if (i >= kDqKStages) mbar_wait(k_empty + sk, ((i / kDqKStages) - 1) & 1, p.st);
         if (i == kDqKStages - 1) mbar_wait(o_done, 0, p.st);
         mbar_expect_tx(k_full + sk, ROW_BYTES);
-        if constexpr (SINKS) {
-          load_key_tile<PANELS, PANEL_BYTES>(k_sm + sk * ROW_BYTES, &tmK, split.k, k_full + sk, h, ksq, i, sink_room(p.sinks), shift);
-        } else {
 #pragma unroll
-          for (int pn = 0; pn < PANELS; ++pn)
-            tma_load_3d(k_sm + sk * ROW_BYTES + pn * PANEL_BYTES, &tmK, k_full + sk, pn * 64, h, ksq + (kt0 + i) * KT);
-        }
+        for (int pn = 0; pn < PANELS; ++pn)
+          tma_load_3d(k_sm + sk * ROW_BYTES + pn * PANEL_BYTES, &tmK, k_full + sk, pn * 64, h, ksq + (kt0 + i) * KT);
         if (i == 0) {
           mbar_expect_tx(qdo_full, ROW_BYTES);
 #pragma unroll
@@ -153,13 +135,9 @@ dense_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         }
         if (i >= kDqVStages) mbar_wait(v_empty + sv, ((i / kDqVStages) - 1) & 1, p.st);
         mbar_expect_tx(v_full + sv, ROW_BYTES);
-        if constexpr (SINKS) {
-          load_key_tile<PANELS, PANEL_BYTES>(v_sm + sv * ROW_BYTES, &tmV, split.v, v_full + sv, h, ksq, i, sink_room(p.sinks), shift);
-        } else {
 #pragma unroll
-          for (int pn = 0; pn < PANELS; ++pn)
-            tma_load_3d(v_sm + sv * ROW_BYTES + pn * PANEL_BYTES, &tmV, v_full + sv, pn * 64, h, ksq + (kt0 + i) * KT);
-        }
+        for (int pn = 0; pn < PANELS; ++pn)
+          tma_load_3d(v_sm + sv * ROW_BYTES + pn * PANEL_BYTES, &tmV, v_full + sv, pn * 64, h, ksq + (kt0 + i) * KT);
         if (i == 0) {
           mbar_expect_tx(o_full, ROW_BYTES);
 #pragma unroll
@@ -184,7 +162,6 @@ dense_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         bool progressed = false;
         if (ns < ntiles && mbar_test(k_full + (ns % kDqKStages), (ns / kDqKStages) & 1) &&
             (ns < 1 || mbar_test(s_empty, (ns - 1) & 1))) {
-          if constexpr (SINKS) clean_key_tile<PANELS, PANEL_BYTES>(k_base + (ns % kDqKStages) * ROW_BYTES, ns, columns, p.sinks, shift);
           tc_fence_after_sync();
           if (elect_one()) {
             umma_block_ss<D / 16, PANEL_BYTES>(tmem, q_addr, k_base + (ns % kDqKStages) * ROW_BYTES, idesc_s);
@@ -209,7 +186,6 @@ dense_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             (np > 0 || mbar_test(qdo_full, 0))) {  // the first dP also needs the dO rows
           tc_fence_after_sync();
           const int sv = np % kDqVStages;
-          if constexpr (SINKS) clean_key_tile<PANELS, PANEL_BYTES>(v_base + sv * ROW_BYTES, np, columns, p.sinks, shift);
           if (elect_one()) {
             umma_block_ss<D / 16, PANEL_BYTES>(tmem + 128, do_addr, v_base + sv * ROW_BYTES, idesc_s);
             umma_commit(v_empty + sv);
@@ -287,12 +263,10 @@ dense_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_empty);
-        const int col0 = (SINKS ? shift + i * KT : (kt0 + i) * KT) + half * 64;  // key of this thread's column 0, in the window
-        const int lim = nvis - col0;  // columns below lim are visible ...
-        const int lo = SINKS || p.left >= 0 ? tpos - p.left - col0 : 0;  // ... from column lo on
-        const int sink = SINKS ? min(p.sinks, nvis) - i * KT - half * 64 : 0;  // ... and those below sink
+        const int lim = nvis - (kt0 + i) * KT - half * 64;  // columns below lim are visible ...
+        const int lo = p.left >= 0 ? tpos - p.left - (kt0 + i) * KT - half * 64 : 0;  // ... from column lo on
         // tiles every row of the warp sees in full (all but those on the mask's edges) skip the mask instructions
-        if (__all_sync(0xffffffffu, lim >= 64 && lo <= (SINKS ? max(sink, 0) : 0))) {
+        if (__all_sync(0xffffffffu, lim >= 64 && lo <= 0)) {
 #pragma unroll
           for (int j = 0; j < 64; j += 2) {
             const float2 x = ffma2(make_float2(__uint_as_float(su[j >> 5][j & 31]), __uint_as_float(su[j >> 5][(j & 31) + 1])),
@@ -303,7 +277,7 @@ dense_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         } else {
 #pragma unroll
           for (int j = 0; j < 64; ++j)
-            pf[j] = masked_exp2((j < lim && j >= lo) || (SINKS && j < sink), fmaf(__uint_as_float(su[j >> 5][j & 31]), p.scale2, nlse));
+            pf[j] = masked_exp2(j < lim && j >= lo, fmaf(__uint_as_float(su[j >> 5][j & 31]), p.scale2, nlse));
         }
       }
       // ---- dS phase ----
@@ -338,7 +312,6 @@ dense_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     // swizzled panel layout the loads use) and writes it with one TMA store per panel: 16-byte stores of one row per lane
     // cost several thousand clocks of the store path per CTA.  Other CTAs (the last of a sequence) store row by row.
     const bool staged = ntiles > 0 && q0 + QT <= Lq;
-    [[maybe_unused]] bool fine = true;
     T* dqrow = static_cast<T*>(p.dq) + (long long)(qs + tpos) * p.dq_sn + (long long)head * p.dq_sh + half * (D / 2);
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) {
@@ -349,10 +322,6 @@ dense_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       } else {
 #pragma unroll
         for (int j = 0; j < 32; ++j) r[j] = 0u;
-      }
-      if constexpr (SINKS) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) fine = fine && fabsf(__uint_as_float(r[j])) < INFINITY;
       }
       if (staged) {
         const uint32_t stage = smem_u32(k_sm);
@@ -378,19 +347,6 @@ dense_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         }
       }
     }
-    if constexpr (SINKS) {
-      // rows with a value that is not finite, one by one; a row is two threads', of warps four apart
-      delta_sh[half * 128 + row] = valid && !fine ? 1.f : 0.f;
-      asm volatile("bar.sync 1, 256;\n" ::: "memory");
-      for (unsigned redo = __ballot_sync(0xffffffffu, half == 0 && delta_sh[row] + delta_sh[128 + row] > 0.f); redo; redo &= redo - 1) {
-        const int src = __ffs(redo) - 1;
-        const int t = __shfl_sync(0xffffffffu, tpos, src), hd = __shfl_sync(0xffffffffu, head, src), rw = __shfl_sync(0xffffffffu, row, src);
-        const float4 x = exact_query_row<T, D, true>(&split, qs, t, hd, h, p.left, p.sinks, p.scale2, p.sm_scale, __shfl_sync(0xffffffffu, lse2, src),
-                                                     __shfl_sync(0xffffffffu, delta, src));
-        if (staged) store_lane_elements_swizzled<T, D, PANEL_BYTES>(k_sm, rw, x);
-        else store_lane_elements<T, D>(static_cast<T*>(p.dq) + (long long)(qs + t) * p.dq_sn + (long long)hd * p.dq_sh, x);
-      }
-    }
     if (staged) {
       fence_proxy_async();  // the TMA engine reads the tile through the async proxy
       asm volatile("bar.sync 1, 256;\n" ::: "memory");
@@ -407,10 +363,9 @@ dense_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
-template <typename T, int D, bool SINKS>
-static int launch_dense_dq(const void* k, const void* v, long long k_sn, long long k_sh, long long v_sn, long long v_sh,
+template <typename T, int D>
+static int launch_dense_dq_tc(const void* k, const void* v, long long k_sn, long long k_sh, long long v_sn, long long v_sh,
                               int total_q, int total_k, int max_seqlen_q, DenseBwdParams p, cudaStream_t stream) {
-  p.rows = total_q;
   CUtensorMap tmQ, tmDO, tmO, tmK, tmV;
   const int QT = 128 / p.G;
   int rc = make_tmap_3d(&tmQ, DT<T>::kTmapType, p.q, D, p.Hq, total_q, p.q_sh, p.q_sn, 64, p.G, QT);
@@ -427,26 +382,12 @@ static int launch_dense_dq(const void* k, const void* v, long long k_sn, long lo
   rc = make_tmap_3d(&tmDQ, DT<T>::kTmapType, p.dq, D, p.Hq, total_q, p.dq_sh, p.dq_sn, 64, p.G, QT);
   if (rc) return rc;
   const size_t smem = (size_t)(2 + kDqKStages + kDqVStages) * (128 * D * 2) + 256 * sizeof(float) + 24 * sizeof(uint64_t) + 16;
-  TileMaps<SINKS> split;
-  if constexpr (SINKS) {
-    const long long ks[8] = {p.q_sn, p.q_sh, k_sn, k_sh, v_sn, v_sh, p.do_sn, p.do_sh};
-    rc = make_sink_maps(split, DT<T>::kTmapType, p.q, k, v, p.dout, ks, D, p.Hkv, total_k, p.sinks);
-    if (rc) return rc;
-  }
-  auto kern = dense_dq_tc_kernel<T, D, SINKS>;
+  auto kern = dense_dq_tc_kernel<T, D>;
   cudaError_t e = allow_smem(kern, smem);
   if (e != cudaSuccess) return cuda_rc(e);
   dim3 grid((max_seqlen_q + QT - 1) / QT, p.B, p.Hkv);
-  if (SINKS) grid = dim3((unsigned)row_tile_slots(total_q, p.B, 7 - p.logG), 1, p.Hkv);
-  { LaunchScope ls_(SINKS ? "sink_dq_tc" : "dense_dq_tc", stream); kern<<<grid, 320, smem, stream>>>(tmQ, tmDO, tmO, tmK, tmV, tmDQ, p, split); }
+  { LaunchScope ls_("dense_dq_tc", stream); kern<<<grid, 320, smem, stream>>>(tmQ, tmDO, tmO, tmK, tmV, tmDQ, p); }
   return cuda_rc(cudaGetLastError());
-}
-
-template <typename T, int D>
-static int launch_dense_dq_tc(const void* k, const void* v, long long k_sn, long long k_sh, long long v_sn, long long v_sh, int total_q, int total_k,
-                              int max_seqlen_q, DenseBwdParams p, cudaStream_t stream) {
-  return p.sinks < 0 ? launch_dense_dq<T, D, false>(k, v, k_sn, k_sh, v_sn, v_sh, total_q, total_k, max_seqlen_q, p, stream)
-                     : launch_dense_dq<T, D, true>(k, v, k_sn, k_sh, v_sn, v_sh, total_q, total_k, max_seqlen_q, p, stream);
 }
 
 int dense_dq_tc(const void* k, const void* v, long long k_sn, long long k_sh, long long v_sn, long long v_sh, int total_q,

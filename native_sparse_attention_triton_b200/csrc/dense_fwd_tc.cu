@@ -60,6 +60,7 @@ struct DenseFwdTcParams {
   Status st;
   int sinks;  // SINKS: ... or key < sinks
   int rows;   // SINKS: of the output
+  uint4* rest;  // SINKS: what its rounding took away (rest_chunk), or nullptr
 };
 
 __device__ __forceinline__ int visible_keys_tc(int t, int Lk, int window, int stride, int causal) {
@@ -180,7 +181,7 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           if (c >= kTcStages) mbar_wait(empty + s, ((c / kTcStages) - 1) & 1, p.st);
           mbar_expect_tx(full + s, KV_BYTES);
           if constexpr (SINKS) {
-            load_key_tile<PANELS, PANEL_BYTES>(sm + s * KV_BYTES, tm, tm == &tmK ? split.k : split.v, full + s, w.head, w.ksq, i, sink_room(p.sinks), w.kt0);
+            load_key_tile<kTcKeyTile, PANELS>(sm + s * KV_BYTES, tm, tm == &tmK ? split.k : split.v, full + s, w.head, w.ksq, i, sink_room(p.sinks), w.kt0);
             return;
           }
 #pragma unroll
@@ -244,7 +245,7 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     // V of tile i of the present item, in stage st, before its products
     auto clean_v = [&](unsigned st, int i) {
       if constexpr (SINKS)
-        clean_key_tile<PANELS, PANEL_BYTES>(v_base + st * KV_BYTES, i, min(w.q0 + 2 * QT, w.Lq) - w.kt0, p.sinks, w.kt0);
+        clean_key_tile<kTcKeyTile, PANELS>(v_base + st * KV_BYTES, i, min(w.q0 + 2 * QT, w.Lq) - w.kt0);
     };
     // S of tile x of the item that starts at row tile t, for its first key tile c
     auto start = [&](unsigned c, unsigned t, int x) {
@@ -329,6 +330,199 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     const int row = (warp & 3) * 32 + lane;
     const uint32_t s_base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(g * 128);
     const uint32_t o_base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 256u + (uint32_t)(g * 128);
+    // O of this thread's row, rescaled
+    auto rescale = [&](float factor) {
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t r[32];
+        tmem_ld32(o_base + c * 32, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const float2 y = fmul2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), make_float2(factor, factor));
+          r[j] = __float_as_uint(y.x);
+          r[j + 1] = __float_as_uint(y.y);
+        }
+        tmem_st32(o_base + c * 32, r);
+      }
+      tmem_st_wait();
+    };
+    // A tile of the list of keys.  One that all rows see in full and that all have a reference maximum for is tried in a single pass, as in
+    // the general code below; any other takes two, maximum and exponentials, in chunks of 32 columns: a chunk that no row of the warp sees
+    // costs nothing, one that all see in full has no mask instructions.  The two passes are loops that are not unrolled: with every
+    // form unrolled four times the instructions did not fit the cache, and a row tile's softmax took 4000 to 10 000 clocks.  There the
+    // output is divided by the sum of the ROUNDED probabilities: where a row sees few keys, one of nearly all the weight then leaves no
+    // rounding in o, which the backward pass's sum o dO needs (rest_chunk); log-sum-exp has the exact sum.
+    [[maybe_unused]] auto sink_softmax_tile = [&](int i, int nvis, int tpos, int shift, float& m_ref, float& l, float& l_rounded, int kt) {
+      const int lim = nvis - shift - i * kTcKeyTile, lo = tpos - p.left - shift - i * kTcKeyTile, sink = min(p.sinks, nvis) - i * kTcKeyTile;
+      auto publish = [&] {
+        tmem_st_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + g);
+      };
+      if (__all_sync(0xffffffffu, lim >= kTcKeyTile && lo <= max(sink, 0) && m_ref != -INFINITY)) {
+        uint32_t pk[64];
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t su[32];
+          tmem_ld32(s_base + c * 32, su);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float2 x = ffma2(make_float2(__uint_as_float(su[2 * j]), __uint_as_float(su[2 * j + 1])), make_float2(p.scale2, p.scale2),
+                                   make_float2(-m_ref, -m_ref));
+            t4[j & 3] = fmax3(t4[j & 3], x.x, x.y);
+            const float2 e = j % kPolyEvery == kPolyEvery - 1 ? exp2_poly2(x) : make_float2(fast_exp2(x.x), fast_exp2(x.y));
+            sum[j & 1] = fadd2(sum[j & 1], e);
+            pk[c * 16 + j] = DT<T>::pack(e.x, e.y);
+          }
+        }
+        if (!__any_sync(0xffffffffu, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) > 8.f)) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pc[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) pc[j] = pk[c * 16 + j];
+            tmem_st16(s_base + c * 16, pc);
+          }
+          const float more = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+          l += more;
+          l_rounded += more;
+          publish();
+          return;
+        }
+      }
+      // the columns of chunk c that this row sees
+      auto seen = [&](int c) {
+        auto below = [&](int x) { return __funnelshift_lc(0xffffffffu, 0u, min(32, max(0, x - c * 32))); };
+        return (below(lim) & ~below(lo)) | below(sink);
+      };
+      float top = -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t see = seen(c);
+        if (!__any_sync(0xffffffffu, see != 0u)) continue;
+        uint32_t su[32];
+        tmem_ld32(s_base + c * 32, su);
+        tmem_ld_wait();
+        if (!__all_sync(0xffffffffu, see == 0xffffffffu)) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) su[j] = see >> j & 1u ? su[j] : __float_as_uint(-INFINITY);
+        }
+        float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) t4[j >> 1 & 3] = fmax3(t4[j >> 1 & 3], __uint_as_float(su[j]), __uint_as_float(su[j + 1]));
+        top = fmax3(top, fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+      }
+      top *= p.scale2;  // (the scale is positive)
+      const bool need = top > m_ref + 8.f;
+      if (__any_sync(0xffffffffu, need)) {
+        float factor = 1.f;
+        if (need) {
+          factor = m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - top);
+          m_ref = top;
+          l *= factor;
+          l_rounded *= factor;
+        }
+        if (i > 0) {
+          mbar_wait(pv_done + g, (kt + i - 1) & 1, p.st);  // P V of the previous key tile is complete: O is stable
+          tc_fence_after_sync();
+          rescale(factor);
+        }
+      }
+      const float nm = m_ref == -INFINITY ? 0.f : -m_ref;
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, rounded[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t see = seen(c);
+        uint32_t pk[16];
+        if (__any_sync(0xffffffffu, see != 0u)) {
+          uint32_t su[32];
+          tmem_ld32(s_base + c * 32, su);
+          tmem_ld_wait();
+          auto exps = [&](auto full_tag) {
+            constexpr bool FULL = decltype(full_tag)::value;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float2 x = ffma2(make_float2(__uint_as_float(su[2 * j]), __uint_as_float(su[2 * j + 1])), make_float2(p.scale2, p.scale2),
+                                     make_float2(nm, nm));
+              float2 e;
+              if (!FULL) e = make_float2(masked_exp2(see >> (2 * j) & 1u, x.x), masked_exp2(see >> (2 * j + 1) & 1u, x.y));
+              else if (j % kPolyEvery == kPolyEvery - 1) e = exp2_poly2(x);
+              else e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+              sum[j & 1] = fadd2(sum[j & 1], e);
+              pk[j] = DT<T>::pack(e.x, e.y);
+              rounded[j & 1] = fadd2(rounded[j & 1], DT<T>::unpack(pk[j]));
+            }
+          };
+          if (__all_sync(0xffffffffu, see == 0xffffffffu)) exps(std::true_type{});
+          else exps(std::false_type{});
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) pk[j] = 0u;
+        }
+        // over the logits: columns [16c, 16c + 16) lie in chunks that have been read
+        tmem_st16(s_base + c * 16, pk);
+      }
+      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      l_rounded += (rounded[0].x + rounded[0].y) + (rounded[1].x + rounded[1].y);
+      publish();
+    };
+    // The output of a row tile, 32 columns at a time.
+    [[maybe_unused]] auto sink_output = [&](const AttnItem& w, int tpos, int head, bool valid, bool staged, int qb, float inv, float lse) {
+      T* orow = static_cast<T*>(p.o) + (long long)(w.qs + tpos) * p.o_sn + (long long)head * p.o_sh;
+      float2 zero = make_float2(0.f, 0.f);
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t r[32];
+        tmem_ld32(o_base + c * 32, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 x = fmul2(make_float2(__uint_as_float(r[q4 * 8 + 2 * e]), __uint_as_float(r[q4 * 8 + 2 * e + 1])), make_float2(inv, inv));
+            zero = ffma2(x, make_float2(0.f, 0.f), zero);
+            hi[e] = DT<T>::pack(x.x, x.y);
+            const float2 h2 = DT<T>::unpack(hi[e]);
+            lo[e] = DT<T>::pack(x.x - h2.x, x.y - h2.y);
+          }
+          const int ci = c * 4 + q4;
+          if (p.rest && valid)
+            p.rest[rest_chunk(ci, w.head, p.Hkv, p.rows, w.qs + tpos, p.G, row & (p.G - 1))] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          if (staged)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(smem_u32(q_sm + qb * Q_BYTES) + row * 128 + (ci >> 3) * PANEL_BYTES +
+                                                                             (((ci & 7) ^ (row & 7)) << 4)),
+                         "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
+          else if (valid)
+            *reinterpret_cast<uint4*>(orow + ci * 8) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        }
+      }
+      tc_fence_before_sync();
+      // rows with a value that is not finite, one by one (0 times infinity is no number)
+      __syncwarp();
+      for (unsigned redo = __ballot_sync(0xffffffffu, valid && zero.x + zero.y != 0.f); redo; redo &= redo - 1) {
+        const int src = __ffs(redo) - 1;
+        const int t = __shfl_sync(0xffffffffu, tpos, src), hd = __shfl_sync(0xffffffffu, head, src), rw = __shfl_sync(0xffffffffu, row, src);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if constexpr (SINKS)
+          x = exact_query_row<T, D, false>(&split, w.qs, t, hd, w.head, p.left, p.sinks, p.scale2, 0.f, __shfl_sync(0xffffffffu, lse, src), 0.f);
+        if (staged) store_lane_elements_swizzled<T, D, PANEL_BYTES>(q_sm + qb * Q_BYTES, rw, x);
+        else store_lane_elements<T, D>(static_cast<T*>(p.o) + (long long)(w.qs + t) * p.o_sn + (long long)hd * p.o_sh, x);
+        if (p.rest) {
+          const int at = lane * (D / 32);  // element; a chunk has eight
+          T* chunk = reinterpret_cast<T*>(p.rest + rest_chunk(at / 8, w.head, p.Hkv, p.rows, w.qs + t, p.G, hd - w.head * p.G));
+          const float2 a = DT<T>::unpack(DT<T>::pack(x.x, x.y)), b = DT<T>::unpack(DT<T>::pack(x.z, x.w));
+          uint32_t* dst = reinterpret_cast<uint32_t*>(chunk + at % 8);
+          dst[0] = DT<T>::pack(x.x - a.x, x.y - a.y);
+          if constexpr (D == 128) dst[1] = DT<T>::pack(x.z - b.x, x.w - b.y);
+        }
+      }
+    };
     int rt = g, kt = 0, taken = 0;  // this warp's row tile, key tiles of the items before the present one, items taken
     AttnItem w;
     while (item_take(ring, taken++, w, p.st)) {
@@ -338,16 +532,19 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       const int nvis = valid ? visible_keys_tc(tpos, w.Lk, p.window, p.stride, p.causal) : 0;
       const int ntiles = w.ntiles;
       float m_ref = -INFINITY, l = 0.f;
+      [[maybe_unused]] float l_rounded = 0.f;
       for (int i = 0; i < ntiles; ++i) {
         mbar_wait(s_full + g, (kt + i) & 1, p.st);
         tc_fence_after_sync();
-        const int col0 = SINKS ? w.kt0 + i * kTcKeyTile : (w.kt0 + i) * kTcKeyTile;  // key of column 0, in the window
-        const int lim = nvis - col0;  // columns below lim are visible ...
-        const int lo = SINKS || p.left >= 0 ? tpos - p.left - col0 : 0;  // ... from column lo on
-        const int sink = SINKS ? min(p.sinks, nvis) - i * kTcKeyTile : 0;  // ... and those below sink
+        if constexpr (SINKS) {
+          sink_softmax_tile(i, nvis, tpos, w.kt0, m_ref, l, l_rounded, kt);
+          continue;
+        }
+        const int lim = nvis - (w.kt0 + i) * kTcKeyTile;  // columns below lim are visible ...
+        const int lo = p.left >= 0 ? tpos - p.left - (w.kt0 + i) * kTcKeyTile : 0;  // ... from column lo on
         // Key tiles that every row of the warp sees in full (all but those on the mask's edge) take a path without the
         // per-element mask instructions.
-        const bool full = __all_sync(0xffffffffu, lim >= kTcKeyTile && lo <= (SINKS ? max(sink, 0) : 0));
+        const bool full = __all_sync(0xffffffffu, lim >= kTcKeyTile && lo <= 0);
         // Full tiles of rows that already have a reference maximum are tried in ONE pass over the logits: exponentials
         // relative to the current reference, with the maximum of the exponents tracked on the side.  If no row of the
         // warp outgrew its reference by more than 2^8 -- the same test the general form makes -- the packed P is stored
@@ -393,12 +590,7 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           // raised) reference.
           auto seen = [&](int c) {
             const int hi_c = min(32, max(0, lim - c * 32)), lo_c = min(32, max(0, lo - c * 32));
-            const uint32_t in = (hi_c < 32 ? (1u << hi_c) - 1u : 0xffffffffu) & ~(lo_c < 32 ? (1u << lo_c) - 1u : 0xffffffffu);
-            if constexpr (SINKS) {
-              const int sk = min(32, max(0, sink - c * 32));
-              return in | (sk < 32 ? (1u << sk) - 1u : 0xffffffffu);
-            }
-            return in;
+            return (hi_c < 32 ? (1u << hi_c) - 1u : 0xffffffffu) & ~(lo_c < 32 ? (1u << lo_c) - 1u : 0xffffffffu);
           };
           float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -428,20 +620,7 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           if (i > 0 && __any_sync(0xffffffffu, need)) {
             mbar_wait(pv_done + g, (kt + i - 1) & 1, p.st);  // P V of the previous key tile is complete: O is stable
             tc_fence_after_sync();
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t r[32];
-              tmem_ld32(o_base + c * 32, r);
-              tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 32; j += 2) {
-                const float2 y = fmul2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), make_float2(factor, factor));
-                r[j] = __float_as_uint(y.x);
-                r[j + 1] = __float_as_uint(y.y);
-              }
-              tmem_st32(o_base + c * 32, r);
-            }
-            tmem_st_wait();
+            rescale(factor);
           }
           // P as 16-bit pairs over the logits: the 32 columns of chunk c become the 16 packed columns [16c, 16c+16), which lie
           // inside the 64 columns already in registers when chunk c is written
@@ -486,7 +665,8 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         if (lane == 0) mbar_arrive(p_full + g);
       }
       // ---- epilogue: O / l ----
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float norm = SINKS ? l_rounded : l;
+      const float inv = norm > 0.f ? 1.f / norm : 0.f;
       if (valid) p.lse[(long long)(w.qs + tpos) * p.Hq + head] = l > 0.f ? m_ref + log2f(l) : -INFINITY;
       // A row tile whose tokens all belong to the sequence leaves through its own Q buffer (free since its last S product, in the
       // swizzled panel layout) and one TMA store per panel; otherwise row by row.
@@ -496,50 +676,37 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         mbar_wait(pv_done + g, (kt + ntiles - 1) & 1, p.st);
         tc_fence_after_sync();
       }
-      T* orow = static_cast<T*>(p.o) + (long long)(w.qs + tpos) * p.o_sn + (long long)head * p.o_sh;
-      const uint32_t stage = smem_u32(q_sm + qb * Q_BYTES) + row * 128;
-      uint32_t r[D / 32][32];
-      if (ntiles > 0) {
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) tmem_ld32(o_base + c * 32, r[c]);
-        tmem_ld_wait();
-        tc_fence_before_sync();
-      } else {
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-          for (int j = 0; j < 32; ++j) r[c][j] = 0u;
-      }
-#pragma unroll
-      for (int ci = 0; ci < D / 8; ++ci) {  // 16-byte chunks of the row
-        const uint32_t* x = r[ci >> 2] + (ci & 3) * 8;
-        uint4 out;
-        out.x = DT<T>::pack(__uint_as_float(x[0]) * inv, __uint_as_float(x[1]) * inv);
-        out.y = DT<T>::pack(__uint_as_float(x[2]) * inv, __uint_as_float(x[3]) * inv);
-        out.z = DT<T>::pack(__uint_as_float(x[4]) * inv, __uint_as_float(x[5]) * inv);
-        out.w = DT<T>::pack(__uint_as_float(x[6]) * inv, __uint_as_float(x[7]) * inv);
-        if (staged) {
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(stage + (ci >> 3) * PANEL_BYTES + (((ci & 7) ^ (row & 7)) << 4)),
-                       "r"(out.x), "r"(out.y), "r"(out.z), "r"(out.w) : "memory");
-        } else if (valid) {
-          *reinterpret_cast<uint4*>(orow + ci * 8) = out;
-        }
-      }
       if constexpr (SINKS) {
-        // rows with a value that is not finite, one by one
-        bool fine = true;
+        sink_output(w, tpos, head, valid, staged, qb, inv, m_ref + log2f(l));
+      } else {
+        T* orow = static_cast<T*>(p.o) + (long long)(w.qs + tpos) * p.o_sn + (long long)head * p.o_sh;
+        const uint32_t stage = smem_u32(q_sm + qb * Q_BYTES) + row * 128;
+        uint32_t r[D / 32][32];
+        if (ntiles > 0) {
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c)
+          for (int c = 0; c < D / 32; ++c) tmem_ld32(o_base + c * 32, r[c]);
+          tmem_ld_wait();
+          tc_fence_before_sync();
+        } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) fine = fine && fabsf(__uint_as_float(r[c][j])) < INFINITY;
-        __syncwarp();
-        for (unsigned redo = __ballot_sync(0xffffffffu, valid && !fine); redo; redo &= redo - 1) {
-          const int src = __ffs(redo) - 1;
-          const int t = __shfl_sync(0xffffffffu, tpos, src), hd = __shfl_sync(0xffffffffu, head, src), rw = __shfl_sync(0xffffffffu, row, src);
-          const float ls = __shfl_sync(0xffffffffu, m_ref + log2f(l), src);
-          const float4 x = exact_query_row<T, D, false>(&split, w.qs, t, hd, w.head, p.left, p.sinks, p.scale2, 0.f, ls, 0.f);
-          if (staged) store_lane_elements_swizzled<T, D, PANEL_BYTES>(q_sm + qb * Q_BYTES, rw, x);
-          else store_lane_elements<T, D>(static_cast<T*>(p.o) + (long long)(w.qs + t) * p.o_sn + (long long)hd * p.o_sh, x);
+          for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[c][j] = 0u;
+        }
+#pragma unroll
+        for (int ci = 0; ci < D / 8; ++ci) {  // 16-byte chunks of the row
+          const uint32_t* x = r[ci >> 2] + (ci & 3) * 8;
+          uint4 out;
+          out.x = DT<T>::pack(__uint_as_float(x[0]) * inv, __uint_as_float(x[1]) * inv);
+          out.y = DT<T>::pack(__uint_as_float(x[2]) * inv, __uint_as_float(x[3]) * inv);
+          out.z = DT<T>::pack(__uint_as_float(x[4]) * inv, __uint_as_float(x[5]) * inv);
+          out.w = DT<T>::pack(__uint_as_float(x[6]) * inv, __uint_as_float(x[7]) * inv);
+          if (staged) {
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(stage + (ci >> 3) * PANEL_BYTES + (((ci & 7) ^ (row & 7)) << 4)),
+                         "r"(out.x), "r"(out.y), "r"(out.z), "r"(out.w) : "memory");
+          } else if (valid) {
+            *reinterpret_cast<uint4*>(orow + ci * 8) = out;
+          }
         }
       }
       if (ntiles > 0) {
@@ -558,12 +725,12 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 
 // The two boxes of a split tile of K and V (none where the sinks fill whole tiles).
 int make_sink_maps(SinkMaps& m, CUtensorMapDataType dt, const void* q, const void* k, const void* v, const void* dout, const long long* S, int D,
-                   int Hkv, int Nk, int sinks) {
+                   int Hkv, int Nk, int sinks, int tile) {
   m.q = q; m.keys = k; m.values = v; m.dout = dout;
   m.q_sn = S[0]; m.q_sh = S[1]; m.k_sn = S[2]; m.k_sh = S[3]; m.v_sn = S[4]; m.v_sh = S[5]; m.do_sn = S[6]; m.do_sh = S[7];
-  const int first = sink_room(sinks) % 128;
+  const int first = sink_room(sinks) % tile;
   for (int x = 0; x < 2; ++x) {
-    const int rows = first == 0 ? 128 : x ? 128 - first : first;
+    const int rows = first == 0 ? tile : x ? tile - first : first;
     int rc = make_tmap_3d(&m.k[x], dt, k, D, Hkv, Nk, S[3], S[2], 64, 1, rows);
     if (!rc) rc = make_tmap_3d(&m.v[x], dt, v, D, Hkv, Nk, S[5], S[4], 64, 1, rows);
     if (rc) return rc;
@@ -588,7 +755,7 @@ static int launch_dense_fwd_tc(const void* q, const void* k, const void* v, cons
   const size_t smem = (kTcQBufs + 2 * kTcStages) * 128 * D * 2 + sizeof(StealSlot) + sizeof(ItemRing) + 24 * sizeof(uint64_t);
   TileMaps<SINKS> split;
   if constexpr (SINKS) {
-    rc = make_sink_maps(split, DT<T>::kTmapType, q, k, v, nullptr, S, D, p.Hkv, Nk, p.sinks);
+    rc = make_sink_maps(split, DT<T>::kTmapType, q, k, v, nullptr, S, D, p.Hkv, Nk, p.sinks, kTcKeyTile);
     if (rc) return rc;
   }
   auto kern = dense_fwd_tc_kernel<T, D, SINKS>;
@@ -607,14 +774,14 @@ static int launch_dense(const void* q, const void* k, const void* v, const long 
 // entry used by nsa_varlen_attn_fwd (dense_fwd.cu) and, with sinks >= 0, by nsa_sink_window_attn_fwd
 int varlen_attn_fwd_tc(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, void* o, float* lse,
                        int total_q, int total_k, int batch, int Hq, int Hkv, int head_dim, int causal,
-                       int window, int stride, int left, int sinks, const long long* strides, float sm_scale, int dtype, cudaStream_t stream) {
+                       int window, int stride, int left, int sinks, void* rest, const long long* strides, float sm_scale, int dtype, cudaStream_t stream) {
   DenseFwdTcParams p;
   p.o = o; p.lse = lse; p.cu_q = cu_q; p.cu_k = cu_k;
   p.o_sn = strides[6]; p.o_sh = strides[7];
   p.B = batch; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
   p.logG = 0;
   while ((1 << p.logG) < p.G) ++p.logG;
-  p.window = window; p.stride = stride; p.causal = causal; p.left = left; p.sinks = sinks; p.rows = total_q;
+  p.window = window; p.stride = stride; p.causal = causal; p.left = left; p.sinks = sinks; p.rows = total_q; p.rest = static_cast<uint4*>(rest);
   p.scale2 = sm_scale * kLog2e;
   p.st.word = status_word();
   return NSA_DISPATCH_T_D(dtype, head_dim, launch_dense, q, k, v, strides, total_q, total_k, p, stream);

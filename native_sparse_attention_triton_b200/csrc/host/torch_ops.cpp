@@ -567,7 +567,7 @@ struct SinkWindowBackward final : SavingNode {
     if (!grads[0].defined()) return out;
     const auto s = unpack();
     at::AutoDispatchBelowADInplaceOrView guard;
-    const Tensor &q = s[0], &k = s[1], &v = s[2], &o = s[3], &lse = s[4], &cu = s[5];
+    const Tensor &q = s[0], &k = s[1], &v = s[2], &o = s[3], &lse = s[4], &cu = s[5], &rest = s[6];
     const int64_t N = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = k.size(1);
     for (int i = 0; i < 3; ++i) out[i] = empty_like_rows(s[i]);
     if (N == 0) return out;
@@ -577,7 +577,7 @@ struct SinkWindowBackward final : SavingNode {
     QkvStrides st;
     st.add(q).add(k).add(v).add(o).add(dout).add(out[0]).add(out[1]).add(out[2]);
     Launch run(q);
-    check_rc(nsa_sink_window_attn_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(dout), ptr<float>(lse), ptr<int>(cu), ptr(out[0]), ptr(out[1]), ptr(out[2]),
+    check_rc(nsa_sink_window_attn_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(rest), ptr(dout), ptr<float>(lse), ptr<int>(cu), ptr(out[0]), ptr(out[1]), ptr(out[2]),
                                       ptr(ws), bytes, (int)N, (int)cu.size(0) - 1, (int)Hq, (int)Hkv, (int)D, left, sinks, st.s, (float)scale,
                                       dtype_code(q), run.stream),
              "nsa_sink_window_attn_bwd");
@@ -604,7 +604,7 @@ Tensor sink_window_attention(const Tensor& q_in, const Tensor& k_in, const Tenso
   one_device(q_in, k_in, v_in, cu);
   const bool graph = needs_graph({q_in, k_in, v_in});
   const int left = (int)std::min<int64_t>(window, INT_MAX / 2), s = (int)std::min<int64_t>(sinks, INT_MAX / 2);
-  Tensor q, k, v, o, lse;
+  Tensor q, k, v, o, lse, rest;
   {
     at::AutoDispatchBelowADInplaceOrView guard;
     q = inner_contiguous(q_in);
@@ -613,12 +613,13 @@ Tensor sink_window_attention(const Tensor& q_in, const Tensor& k_in, const Tenso
     const int64_t N = q.size(0), Hq = q.size(1), D = q.size(2);
     o = empty({N, Hq, D}, q.scalar_type(), q.device());
     lse = empty({N, Hq}, at::kFloat, q.device());
+    if (graph) rest = empty({N * Hq * D}, q.scalar_type(), q.device());
     if (N > 0) {
       QkvStrides st;
       st.add(q).add(k).add(v).add(o);
       Launch run(q);
-      check_rc(nsa_sink_window_attn_fwd(ptr(q), ptr(k), ptr(v), ptr<int>(cu), ptr(o), ptr<float>(lse), (int)N, (int)cu.size(0) - 1, (int)Hq,
-                                        (int)k.size(1), (int)D, left, s, st.s, (float)scale, dtype_code(q), run.stream),
+      check_rc(nsa_sink_window_attn_fwd(ptr(q), ptr(k), ptr(v), ptr<int>(cu), ptr(o), graph ? ptr(rest) : nullptr, ptr<float>(lse), (int)N,
+                                        (int)cu.size(0) - 1, (int)Hq, (int)k.size(1), (int)D, left, s, st.s, (float)scale, dtype_code(q), run.stream),
                "nsa_sink_window_attn_fwd");
     }
   }
@@ -630,7 +631,7 @@ Tensor sink_window_attention(const Tensor& q_in, const Tensor& k_in, const Tenso
     torch::autograd::set_history(o, node);
     for (const Tensor& t : {q, k, v}) node->saved.push_back(save_input(t));
     node->saved.push_back(SavedVariable(o, /*is_output=*/true));
-    for (const Tensor& t : {lse, cu}) node->saved.push_back(save_input(t));
+    for (const Tensor& t : {lse, cu, rest}) node->saved.push_back(save_input(t));
   }
   return o;
 }

@@ -1,7 +1,7 @@
 // The keys that rows of a sliding window with sinks see, without the gap between the two.
 //
-// Query t of a sequence sees key j <= t iff t - j <= left or j < sinks.  A group of rows at tokens q0, q0 + 1, ... takes its keys in tiles of
-// 128 from the list
+// Query t of a sequence sees key j <= t iff t - j <= left or j < sinks.  A group of rows at tokens q0, q0 + 1, ... takes its keys in tiles
+// (128 forward, 64 backward) from the list
 //     column u:  key u                for u < room,      room = sinks rounded up to 8 rows (the swizzle's unit),
 //                key u + shift        for u >= room,     shift = max(0, q0 - left - room),
 // so the window starts at the first key that any of the rows sees, wherever that lies, and the sinks fill the head of the first tile
@@ -14,7 +14,7 @@
 
 namespace nsa {
 
-// Boxes of the two parts of the tile in which the list jumps: room % 128 rows, and the rest; and the tensors themselves, for the rows that
+// Boxes of the two parts of the tile in which the list jumps: room % (rows of a tile), and the rest; and the tensors themselves, for the rows that
 // are computed one by one (sink_exact.cuh).
 struct SinkMaps {
   CUtensorMap k[2], v[2];
@@ -28,30 +28,37 @@ using TileMaps = std::conditional_t<SINKS, SinkMaps, NoMaps>;
 __host__ __device__ __forceinline__ int sink_room(int sinks) { return (sinks + 7) & ~7; }
 __device__ __forceinline__ int sink_shift(int q0, int left, int room) { return max(0, q0 - left - room); }
 
-// Tile i of the list into shared memory, PANELS panels of PANEL bytes; one thread, with the barrier's bytes announced.  `row0` is the
-// sequence's first key row, `whole` the map with boxes of 128 rows, `part` those of the split tile.
-template <int PANELS, int PANEL>
+// Tile i of the list, KEYS rows of PANELS panels, into shared memory; one thread, with the barrier's bytes announced.  `row0` is the
+// sequence's first key row, `whole` the map with boxes of KEYS rows, `part` those of the split tile.
+template <int KEYS, int PANELS>
 __device__ __forceinline__ void load_key_tile(uint8_t* sm, const CUtensorMap* whole, const CUtensorMap* part, uint64_t* bar, int head, int row0, int i,
                                               int room, int shift) {
-  const int u = i * 128, first = room - u;  // rows of the tile in front of the jump
+  const int u = i * KEYS, first = room - u;  // rows of the tile in front of the jump
 #pragma unroll
   for (int pn = 0; pn < PANELS; ++pn) {
-    if (shift == 0 || first <= 0 || first >= 128) {
-      tma_load_3d(sm + pn * PANEL, whole, bar, pn * 64, head, row0 + u + (first <= 0 ? shift : 0));
+    uint8_t* dst = sm + pn * KEYS * 128;
+    if (shift == 0 || first <= 0 || first >= KEYS) {
+      tma_load_3d(dst, whole, bar, pn * 64, head, row0 + u + (first <= 0 ? shift : 0));
     } else {
-      tma_load_3d(sm + pn * PANEL, part, bar, pn * 64, head, row0 + u);
-      tma_load_3d(sm + pn * PANEL + first * 128, part + 1, bar, pn * 64, head, row0 + room + shift);
+      tma_load_3d(dst, part, bar, pn * 64, head, row0 + u);
+      tma_load_3d(dst + first * 128, part + 1, bar, pn * 64, head, row0 + room + shift);
     }
   }
 }
 
-// The rows of tile i that stand for no key of the rows' list: behind its last column `n`, and between the sinks and the window.
-template <int PANELS, int PANEL>
-__device__ __forceinline__ void clean_key_tile(uint32_t tile, int i, int n, int sinks, int shift) {
-  const int end = n - i * 128;
-  if (end < 128) zero_tile_rows<PANELS, PANEL>(tile, max(0, end), 128);
-  const int hide0 = sinks - i * 128, hide1 = sink_room(sinks) - i * 128;
-  if (shift > 0 && hide1 > hide0 && hide0 < 128 && hide1 > 0) zero_tile_rows<PANELS, PANEL>(tile, max(0, hide0), min(128, hide1));
+// The rows of tile i behind the list's last column n, which are other sequences' or nobody's, as zeros.  (Rows that are not finite are computed
+// again one by one in any case, see sink_exact.cuh; but what lies behind a batch may well not be, and should not cost that.)
+template <int KEYS, int PANELS>
+__device__ __forceinline__ void clean_key_tile(uint32_t tile, int i, int n) {
+  const int end = n - i * KEYS;
+  if (end < KEYS) zero_tile_rows<PANELS, KEYS * 128>(tile, max(0, end), KEYS);
+}
+
+// What the rounding of the output o took away, rounded itself (o is then known to 2^-17, or 2^-22 in fp16): 16-byte chunk c of a row, in an
+// order in which the rows of a warp are neighbours.  The backward pass needs sum_d o dO next to single dO v: where a row looks at few keys the
+// two all but cancel, and what is left of o's rounding becomes as large as dS (one key of weight 1 - w: dS is w of its parts).
+__device__ __forceinline__ long long rest_chunk(int c, int kvh, int Hkv, int rows, int n, int G, int g) {
+  return (((long long)c * Hkv + kvh) * rows + n) * G + g;
 }
 
 // Rows of G heads from `head` on that belong to no sequence (a padded batch), [first, rows), as zeros; block x of n takes every n-th.  A warp.

@@ -109,8 +109,8 @@ def test_evictions_that_are_refused(change):
 def test_c_interface_refuses_before_it_touches_a_device():
     lib = _lib.lib()
     z = _lib.strides_array(*[8] * 16)
-    assert lib.nsa_sink_window_attn_fwd(None, None, None, None, None, None, 1, 1, 1, 1, 128, 1, 1, z, 1.0, 0, None) == -1
-    assert lib.nsa_sink_window_attn_bwd(*[None] * 11, 0, 1, 1, 1, 1, 128, 1, 1, z, 1.0, 0, None) == -1
+    assert lib.nsa_sink_window_attn_fwd(*[None] * 7, 1, 1, 1, 1, 128, 1, 1, z, 1.0, 0, None) == -1
+    assert lib.nsa_sink_window_attn_bwd(*[None] * 12, 0, 1, 1, 1, 1, 128, 1, 1, z, 1.0, 0, None) == -1
     assert lib.nsa_paged_kv_append(*[None] * 8, 1, 1, 1, 128, 1, 1, 1, z, None) == -1
     assert lib.nsa_paged_attn_decode(*[None] * 8, 0, 1, 1, 1, 128, 1, 1, 1, 0, 0, z, 1.0, 0, None) == -1
     assert lib.nsa_paged_kv_evict(*[None] * 9, 1, 1, 128, 1, 1, 1, 1, 1, 1, 0, 0, z, None) == -1
@@ -120,8 +120,8 @@ def test_c_interface_refuses_before_it_touches_a_device():
     assert lib.nsa_paged_kv_append(*[p] * 8, 1, 1, 1, 96, 1, 1, 1, z, None) == -2
     assert lib.nsa_paged_kv_evict(*[p] * 9, 1, 1, 128, 1, 1, 1, 1, 1, 4, 5, 0, z, None) == -1                       # sinks beyond the budget
     odd = _lib.strides_array(*[4] * 16)
-    assert lib.nsa_sink_window_attn_fwd(*[p] * 6, 1, 1, 1, 1, 128, 1, 1, odd, 1.0, 0, None) == -1
-    assert lib.nsa_sink_window_attn_bwd(*[p] * 11, 0, 1, 1, 1, 1, 128, 1, 1, z, 1.0, 0, None) == -3
+    assert lib.nsa_sink_window_attn_fwd(*[p] * 7, 1, 1, 1, 1, 128, 1, 1, odd, 1.0, 0, None) == -1
+    assert lib.nsa_sink_window_attn_bwd(*[p] * 12, 0, 1, 1, 1, 1, 128, 1, 1, z, 1.0, 0, None) == -3
 
 
 def test_reference_gradients_against_differences():

@@ -10,24 +10,21 @@
 #include "host_util.h"
 #include "nsa_b200.h"
 
-#include <algorithm>
-
 namespace nsa {
 
 // tcgen05 implementation (dense_fwd_tc.cu)
 int varlen_attn_fwd_tc(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, void* o, float* lse,
                        int total_q, int total_k, int batch, int Hq, int Hkv, int head_dim, int causal,
-                       int window, int stride, int left, int sinks, void* rest, const long long* strides, float sm_scale, int dtype, cudaStream_t stream);
+                       int window, int stride, int left, const long long* strides, float sm_scale, int dtype, cudaStream_t stream);
 
 }  // namespace nsa
 
-// left >= 0 adds the lower bound key >= t - left (sliding window); only with the plain causal mask and on the tcgen05 kernel.  sinks >= 0
-// lets the first keys of a sequence past it.
+// left >= 0 adds the lower bound key >= t - left (sliding window); only with the plain causal mask and on the tcgen05 kernel
 static int varlen_attn_fwd_common(const void* q, const void* k, const void* v, const int* cu_seqlens_q,
                                   const int* cu_seqlens_k, void* o, float* lse, int total_q, int total_k, int batch,
                                   int max_seqlen_q, int num_q_heads, int num_kv_heads, int head_dim, int causal,
-                                  int window, int stride, int left, int sinks, void* rest, const long long* strides,
-                                  float sm_scale, int dtype, void* stream) {
+                                  int window, int stride, int left, const long long* strides, float sm_scale, int dtype,
+                                  void* stream) {
   using namespace nsa;
   if (left >= 0 && (!causal || window != 1 || stride != 1)) return kUnsupported;
   if (!q || !cu_seqlens_q || !cu_seqlens_k || !o || !lse || !strides) return kInvalid;
@@ -42,7 +39,7 @@ static int varlen_attn_fwd_common(const void* q, const void* k, const void* v, c
   // strides: q_n q_h k_n k_h v_n v_h o_n o_h (those of k and v are checked with their tensor maps)
   if ((strides[0] | strides[1] | strides[6] | strides[7]) % 8 || !aligned16(q) || !aligned16(o)) return kInvalid;
   return varlen_attn_fwd_tc(q, k, v, cu_seqlens_q, cu_seqlens_k, o, lse, total_q, total_k, batch, num_q_heads,
-                            num_kv_heads, head_dim, causal, window, stride, left, sinks, rest, strides, sm_scale, dtype,
+                            num_kv_heads, head_dim, causal, window, stride, left, strides, sm_scale, dtype,
                             static_cast<cudaStream_t>(stream));
 }
 
@@ -52,7 +49,7 @@ extern "C" int nsa_varlen_attn_fwd(const void* q, const void* k, const void* v, 
                                    int window, int stride, const long long* strides, float sm_scale, int dtype,
                                    void* stream) {
   return varlen_attn_fwd_common(q, k, v, cu_seqlens_q, cu_seqlens_k, o, lse, total_q, total_k, batch, max_seqlen_q, num_q_heads,
-                                num_kv_heads, head_dim, causal, window, stride, -1, -1, nullptr, strides, sm_scale, dtype, stream);
+                                num_kv_heads, head_dim, causal, window, stride, -1, strides, sm_scale, dtype, stream);
 }
 
 extern "C" int nsa_window_attn_fwd(const void* q, const void* k, const void* v, const int* cu_seqlens, void* o, float* lse,
@@ -60,15 +57,5 @@ extern "C" int nsa_window_attn_fwd(const void* q, const void* k, const void* v, 
                                    int window_left, const long long* strides, float sm_scale, int dtype, void* stream) {
   if (window_left < 0) return nsa::kInvalid;
   return varlen_attn_fwd_common(q, k, v, cu_seqlens, cu_seqlens, o, lse, total_len, total_len, batch, max_seqlen, num_q_heads,
-                                num_kv_heads, head_dim, 1, 1, 1, window_left, -1, nullptr, strides, sm_scale, dtype, stream);
-}
-
-extern "C" int nsa_sink_window_attn_fwd(const void* q, const void* k, const void* v, const int* cu_seqlens, void* o, void* o_rest, float* lse,
-                                        int total_len, int batch, int num_q_heads, int num_kv_heads, int head_dim, int window_left, int num_sinks,
-                                        const long long* strides, float sm_scale, int dtype, void* stream) {
-  if (window_left < 0 || num_sinks < 0 || !strides || (strides[2] | strides[3] | strides[4] | strides[5]) % 8 || !nsa::aligned16(o_rest)) return nsa::kInvalid;
-  // no query is further from a key than the batch is long
-  return varlen_attn_fwd_common(q, k, v, cu_seqlens, cu_seqlens, o, lse, total_len, total_len, batch, total_len, num_q_heads, num_kv_heads,
-                                head_dim, 1, 1, 1, std::min(window_left, total_len), std::min(num_sinks, total_len), o_rest, strides, sm_scale,
-                                dtype, stream);
+                                num_kv_heads, head_dim, 1, 1, 1, window_left, strides, sm_scale, dtype, stream);
 }

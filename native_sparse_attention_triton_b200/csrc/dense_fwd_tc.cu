@@ -35,8 +35,6 @@
 #include "dispatch.h"
 #include "host_util.h"
 #include "nsa_b200.h"
-#include "sink_exact.cuh"
-#include "sink_keys.cuh"
 #include "tc5.cuh"
 #include "work_steal.cuh"
 
@@ -58,9 +56,6 @@ struct DenseFwdTcParams {
   int left;  // >= 0: sliding window, a query also needs key >= t - left (plain causal mask only); < 0: no lower bound
   float scale2;
   Status st;
-  int sinks;  // SINKS: ... or key < sinks
-  int rows;   // SINKS: of the output
-  uint4* rest;  // SINKS: what its rounding took away (rest_chunk), or nullptr
 };
 
 __device__ __forceinline__ int visible_keys_tc(int t, int Lk, int window, int stride, int causal) {
@@ -75,12 +70,10 @@ constexpr int kTcQBufs = 3;         // row tiles of Q
 constexpr int kTcSoftWarps = 8;     // 4 per row tile
 constexpr int kTcThreads = (kTcSoftWarps + 3) * 32;
 
-// SINKS: a sliding window with sinks; an item's key tiles are those of its list of keys (sink_keys.cuh), whose shift stands in the item's kt0.
-template <typename T, int D, bool SINKS>
+template <typename T, int D>
 __global__ void __launch_bounds__(kTcThreads, 1)
 dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, DenseFwdTcParams p,
-                    const __grid_constant__ TileMaps<SINKS> split) {
+                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, DenseFwdTcParams p) {
   constexpr int PANELS = D / 64;
   constexpr int PANEL_BYTES = 128 * 128;            // 128 rows x 128 B
   constexpr int Q_BYTES = 128 * D * 2;              // one row tile
@@ -147,7 +140,6 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     int kt = 0;    // key tiles so far
     auto lookup = [&](uint3 blk, AttnItem& w) {
       int b, tile;
-      if constexpr (SINKS) zero_rows_behind<T, D>(p.o, p.o_sn, p.o_sh, __ldg(p.cu_q + p.B), p.rows, blk.x, gridDim.x, blk.y * p.G, p.G);
       // long rows first
       if (!find_row_tile(p.cu_q, p.B, 8 - p.logG, (int)gridDim.x - 1 - (int)blk.x, b, w.qs, w.Lq, tile)) return false;
       w.head = blk.y;
@@ -155,11 +147,6 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       w.Lk = __ldg(p.cu_k + b + 1) - w.ksq;
       w.q0 = tile * 2 * QT;
       const int t_hi = min(w.q0 + 2 * QT, w.Lq) - 1;
-      if constexpr (SINKS) {
-        w.kt0 = sink_shift(w.q0, p.left, sink_room(p.sinks));
-        w.ntiles = (t_hi + 1 - w.kt0 + kTcKeyTile - 1) / kTcKeyTile;
-        return true;
-      }
       // with a sliding window the first key tiles are invisible to every row of the item: start at tile kt0
       w.kt0 = p.left >= 0 ? max(0, w.q0 - p.left) / kTcKeyTile : 0;
       w.ntiles = max(0, (visible_keys_tc(t_hi, w.Lk, p.window, p.stride, p.causal) + kTcKeyTile - 1) / kTcKeyTile - w.kt0);
@@ -180,10 +167,6 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           const int c = kt + i, s = c % kTcStages;
           if (c >= kTcStages) mbar_wait(empty + s, ((c / kTcStages) - 1) & 1, p.st);
           mbar_expect_tx(full + s, KV_BYTES);
-          if constexpr (SINKS) {
-            load_key_tile<kTcKeyTile, PANELS>(sm + s * KV_BYTES, tm, tm == &tmK ? split.k : split.v, full + s, w.head, w.ksq, i, sink_room(p.sinks), w.kt0);
-            return;
-          }
 #pragma unroll
           for (int pn = 0; pn < PANELS; ++pn)
             tma_load_3d(sm + s * KV_BYTES + pn * PANEL_BYTES, tm, full + s, pn * 64, w.head, w.ksq + (w.kt0 + i) * kTcKeyTile);
@@ -242,11 +225,6 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       }
     };
     auto q_tile = [&](unsigned t) { return q_base + t % kTcQBufs * Q_BYTES; };
-    // V of tile i of the present item, in stage st, before its products
-    auto clean_v = [&](unsigned st, int i) {
-      if constexpr (SINKS)
-        clean_key_tile<kTcKeyTile, PANELS>(v_base + st * KV_BYTES, i, min(w.q0 + 2 * QT, w.Lq) - w.kt0);
-    };
     // S of tile x of the item that starts at row tile t, for its first key tile c
     auto start = [&](unsigned c, unsigned t, int x) {
       if (x == 0) mbar_wait(k_full + c % kTcStages, (c / kTcStages) & 1, p.st);
@@ -270,7 +248,6 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       for (int i = 0; i + 1 < ntiles; ++i, ++c) {
         const unsigned n = c + 1;
         mbar_wait(v_full + c % kTcStages, (c / kTcStages) & 1, p.st);
-        clean_v(c % kTcStages, i);
         mbar_wait(k_full + n % kTcStages, (n / kTcStages) & 1, p.st);
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
@@ -288,10 +265,7 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 #pragma unroll 1
       for (int g = 0; g < 2; ++g) {
         mbar_wait(p_full + g, c & 1, p.st);
-        if (g == 0) {
-          mbar_wait(v_full + c % kTcStages, (c / kTcStages) & 1, p.st);
-          clean_v(c % kTcStages, ntiles - 1);
-        }
+        if (g == 0) mbar_wait(v_full + c % kTcStages, (c / kTcStages) & 1, p.st);
         tc_fence_after_sync();
         issue_pv(c % kTcStages, g, ntiles == 1);
         if (have < 0) have = next_item(g == 1);
@@ -330,199 +304,6 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     const int row = (warp & 3) * 32 + lane;
     const uint32_t s_base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(g * 128);
     const uint32_t o_base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 256u + (uint32_t)(g * 128);
-    // O of this thread's row, rescaled
-    auto rescale = [&](float factor) {
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t r[32];
-        tmem_ld32(o_base + c * 32, r);
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          const float2 y = fmul2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), make_float2(factor, factor));
-          r[j] = __float_as_uint(y.x);
-          r[j + 1] = __float_as_uint(y.y);
-        }
-        tmem_st32(o_base + c * 32, r);
-      }
-      tmem_st_wait();
-    };
-    // A tile of the list of keys.  One that all rows see in full and that all have a reference maximum for is tried in a single pass, as in
-    // the general code below; any other takes two, maximum and exponentials, in chunks of 32 columns: a chunk that no row of the warp sees
-    // costs nothing, one that all see in full has no mask instructions.  The two passes are loops that are not unrolled: with every
-    // form unrolled four times the instructions did not fit the cache, and a row tile's softmax took 4000 to 10 000 clocks.  There the
-    // output is divided by the sum of the ROUNDED probabilities: where a row sees few keys, one of nearly all the weight then leaves no
-    // rounding in o, which the backward pass's sum o dO needs (rest_chunk); log-sum-exp has the exact sum.
-    [[maybe_unused]] auto sink_softmax_tile = [&](int i, int nvis, int tpos, int shift, float& m_ref, float& l, float& l_rounded, int kt) {
-      const int lim = nvis - shift - i * kTcKeyTile, lo = tpos - p.left - shift - i * kTcKeyTile, sink = min(p.sinks, nvis) - i * kTcKeyTile;
-      auto publish = [&] {
-        tmem_st_wait();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + g);
-      };
-      if (__all_sync(0xffffffffu, lim >= kTcKeyTile && lo <= max(sink, 0) && m_ref != -INFINITY)) {
-        uint32_t pk[64];
-        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t su[32];
-          tmem_ld32(s_base + c * 32, su);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float2 x = ffma2(make_float2(__uint_as_float(su[2 * j]), __uint_as_float(su[2 * j + 1])), make_float2(p.scale2, p.scale2),
-                                   make_float2(-m_ref, -m_ref));
-            t4[j & 3] = fmax3(t4[j & 3], x.x, x.y);
-            const float2 e = j % kPolyEvery == kPolyEvery - 1 ? exp2_poly2(x) : make_float2(fast_exp2(x.x), fast_exp2(x.y));
-            sum[j & 1] = fadd2(sum[j & 1], e);
-            pk[c * 16 + j] = DT<T>::pack(e.x, e.y);
-          }
-        }
-        if (!__any_sync(0xffffffffu, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) > 8.f)) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t pc[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) pc[j] = pk[c * 16 + j];
-            tmem_st16(s_base + c * 16, pc);
-          }
-          const float more = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-          l += more;
-          l_rounded += more;
-          publish();
-          return;
-        }
-      }
-      // the columns of chunk c that this row sees
-      auto seen = [&](int c) {
-        auto below = [&](int x) { return __funnelshift_lc(0xffffffffu, 0u, min(32, max(0, x - c * 32))); };
-        return (below(lim) & ~below(lo)) | below(sink);
-      };
-      float top = -INFINITY;
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        const uint32_t see = seen(c);
-        if (!__any_sync(0xffffffffu, see != 0u)) continue;
-        uint32_t su[32];
-        tmem_ld32(s_base + c * 32, su);
-        tmem_ld_wait();
-        if (!__all_sync(0xffffffffu, see == 0xffffffffu)) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) su[j] = see >> j & 1u ? su[j] : __float_as_uint(-INFINITY);
-        }
-        float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int j = 0; j < 32; j += 2) t4[j >> 1 & 3] = fmax3(t4[j >> 1 & 3], __uint_as_float(su[j]), __uint_as_float(su[j + 1]));
-        top = fmax3(top, fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-      }
-      top *= p.scale2;  // (the scale is positive)
-      const bool need = top > m_ref + 8.f;
-      if (__any_sync(0xffffffffu, need)) {
-        float factor = 1.f;
-        if (need) {
-          factor = m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - top);
-          m_ref = top;
-          l *= factor;
-          l_rounded *= factor;
-        }
-        if (i > 0) {
-          mbar_wait(pv_done + g, (kt + i - 1) & 1, p.st);  // P V of the previous key tile is complete: O is stable
-          tc_fence_after_sync();
-          rescale(factor);
-        }
-      }
-      const float nm = m_ref == -INFINITY ? 0.f : -m_ref;
-      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, rounded[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        const uint32_t see = seen(c);
-        uint32_t pk[16];
-        if (__any_sync(0xffffffffu, see != 0u)) {
-          uint32_t su[32];
-          tmem_ld32(s_base + c * 32, su);
-          tmem_ld_wait();
-          auto exps = [&](auto full_tag) {
-            constexpr bool FULL = decltype(full_tag)::value;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float2 x = ffma2(make_float2(__uint_as_float(su[2 * j]), __uint_as_float(su[2 * j + 1])), make_float2(p.scale2, p.scale2),
-                                     make_float2(nm, nm));
-              float2 e;
-              if (!FULL) e = make_float2(masked_exp2(see >> (2 * j) & 1u, x.x), masked_exp2(see >> (2 * j + 1) & 1u, x.y));
-              else if (j % kPolyEvery == kPolyEvery - 1) e = exp2_poly2(x);
-              else e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-              sum[j & 1] = fadd2(sum[j & 1], e);
-              pk[j] = DT<T>::pack(e.x, e.y);
-              rounded[j & 1] = fadd2(rounded[j & 1], DT<T>::unpack(pk[j]));
-            }
-          };
-          if (__all_sync(0xffffffffu, see == 0xffffffffu)) exps(std::true_type{});
-          else exps(std::false_type{});
-        } else {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) pk[j] = 0u;
-        }
-        // over the logits: columns [16c, 16c + 16) lie in chunks that have been read
-        tmem_st16(s_base + c * 16, pk);
-      }
-      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-      l_rounded += (rounded[0].x + rounded[0].y) + (rounded[1].x + rounded[1].y);
-      publish();
-    };
-    // The output of a row tile, 32 columns at a time.
-    [[maybe_unused]] auto sink_output = [&](const AttnItem& w, int tpos, int head, bool valid, bool staged, int qb, float inv, float lse) {
-      T* orow = static_cast<T*>(p.o) + (long long)(w.qs + tpos) * p.o_sn + (long long)head * p.o_sh;
-      float2 zero = make_float2(0.f, 0.f);
-#pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t r[32];
-        tmem_ld32(o_base + c * 32, r);
-        tmem_ld_wait();
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          uint32_t hi[4], lo[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 x = fmul2(make_float2(__uint_as_float(r[q4 * 8 + 2 * e]), __uint_as_float(r[q4 * 8 + 2 * e + 1])), make_float2(inv, inv));
-            zero = ffma2(x, make_float2(0.f, 0.f), zero);
-            hi[e] = DT<T>::pack(x.x, x.y);
-            const float2 h2 = DT<T>::unpack(hi[e]);
-            lo[e] = DT<T>::pack(x.x - h2.x, x.y - h2.y);
-          }
-          const int ci = c * 4 + q4;
-          if (p.rest && valid)
-            p.rest[rest_chunk(ci, w.head, p.Hkv, p.rows, w.qs + tpos, p.G, row & (p.G - 1))] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          if (staged)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(smem_u32(q_sm + qb * Q_BYTES) + row * 128 + (ci >> 3) * PANEL_BYTES +
-                                                                             (((ci & 7) ^ (row & 7)) << 4)),
-                         "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
-          else if (valid)
-            *reinterpret_cast<uint4*>(orow + ci * 8) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        }
-      }
-      tc_fence_before_sync();
-      // rows with a value that is not finite, one by one (0 times infinity is no number)
-      __syncwarp();
-      for (unsigned redo = __ballot_sync(0xffffffffu, valid && zero.x + zero.y != 0.f); redo; redo &= redo - 1) {
-        const int src = __ffs(redo) - 1;
-        const int t = __shfl_sync(0xffffffffu, tpos, src), hd = __shfl_sync(0xffffffffu, head, src), rw = __shfl_sync(0xffffffffu, row, src);
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if constexpr (SINKS)
-          x = exact_query_row<T, D, false>(&split, w.qs, t, hd, w.head, p.left, p.sinks, p.scale2, 0.f, __shfl_sync(0xffffffffu, lse, src), 0.f);
-        if (staged) store_lane_elements_swizzled<T, D, PANEL_BYTES>(q_sm + qb * Q_BYTES, rw, x);
-        else store_lane_elements<T, D>(static_cast<T*>(p.o) + (long long)(w.qs + t) * p.o_sn + (long long)hd * p.o_sh, x);
-        if (p.rest) {
-          const int at = lane * (D / 32);  // element; a chunk has eight
-          T* chunk = reinterpret_cast<T*>(p.rest + rest_chunk(at / 8, w.head, p.Hkv, p.rows, w.qs + t, p.G, hd - w.head * p.G));
-          const float2 a = DT<T>::unpack(DT<T>::pack(x.x, x.y)), b = DT<T>::unpack(DT<T>::pack(x.z, x.w));
-          uint32_t* dst = reinterpret_cast<uint32_t*>(chunk + at % 8);
-          dst[0] = DT<T>::pack(x.x - a.x, x.y - a.y);
-          if constexpr (D == 128) dst[1] = DT<T>::pack(x.z - b.x, x.w - b.y);
-        }
-      }
-    };
     int rt = g, kt = 0, taken = 0;  // this warp's row tile, key tiles of the items before the present one, items taken
     AttnItem w;
     while (item_take(ring, taken++, w, p.st)) {
@@ -532,14 +313,9 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       const int nvis = valid ? visible_keys_tc(tpos, w.Lk, p.window, p.stride, p.causal) : 0;
       const int ntiles = w.ntiles;
       float m_ref = -INFINITY, l = 0.f;
-      [[maybe_unused]] float l_rounded = 0.f;
       for (int i = 0; i < ntiles; ++i) {
         mbar_wait(s_full + g, (kt + i) & 1, p.st);
         tc_fence_after_sync();
-        if constexpr (SINKS) {
-          sink_softmax_tile(i, nvis, tpos, w.kt0, m_ref, l, l_rounded, kt);
-          continue;
-        }
         const int lim = nvis - (w.kt0 + i) * kTcKeyTile;  // columns below lim are visible ...
         const int lo = p.left >= 0 ? tpos - p.left - (w.kt0 + i) * kTcKeyTile : 0;  // ... from column lo on
         // Key tiles that every row of the warp sees in full (all but those on the mask's edge) take a path without the
@@ -620,7 +396,20 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           if (i > 0 && __any_sync(0xffffffffu, need)) {
             mbar_wait(pv_done + g, (kt + i - 1) & 1, p.st);  // P V of the previous key tile is complete: O is stable
             tc_fence_after_sync();
-            rescale(factor);
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t r[32];
+              tmem_ld32(o_base + c * 32, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {
+                const float2 y = fmul2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), make_float2(factor, factor));
+                r[j] = __float_as_uint(y.x);
+                r[j + 1] = __float_as_uint(y.y);
+              }
+              tmem_st32(o_base + c * 32, r);
+            }
+            tmem_st_wait();
           }
           // P as 16-bit pairs over the logits: the 32 columns of chunk c become the 16 packed columns [16c, 16c+16), which lie
           // inside the 64 columns already in registers when chunk c is written
@@ -665,8 +454,7 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         if (lane == 0) mbar_arrive(p_full + g);
       }
       // ---- epilogue: O / l ----
-      const float norm = SINKS ? l_rounded : l;
-      const float inv = norm > 0.f ? 1.f / norm : 0.f;
+      const float inv = l > 0.f ? 1.f / l : 0.f;
       if (valid) p.lse[(long long)(w.qs + tpos) * p.Hq + head] = l > 0.f ? m_ref + log2f(l) : -INFINITY;
       // A row tile whose tokens all belong to the sequence leaves through its own Q buffer (free since its last S product, in the
       // swizzled panel layout) and one TMA store per panel; otherwise row by row.
@@ -676,37 +464,33 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         mbar_wait(pv_done + g, (kt + ntiles - 1) & 1, p.st);
         tc_fence_after_sync();
       }
-      if constexpr (SINKS) {
-        sink_output(w, tpos, head, valid, staged, qb, inv, m_ref + log2f(l));
+      T* orow = static_cast<T*>(p.o) + (long long)(w.qs + tpos) * p.o_sn + (long long)head * p.o_sh;
+      const uint32_t stage = smem_u32(q_sm + qb * Q_BYTES) + row * 128;
+      uint32_t r[D / 32][32];
+      if (ntiles > 0) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) tmem_ld32(o_base + c * 32, r[c]);
+        tmem_ld_wait();
+        tc_fence_before_sync();
       } else {
-        T* orow = static_cast<T*>(p.o) + (long long)(w.qs + tpos) * p.o_sn + (long long)head * p.o_sh;
-        const uint32_t stage = smem_u32(q_sm + qb * Q_BYTES) + row * 128;
-        uint32_t r[D / 32][32];
-        if (ntiles > 0) {
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) tmem_ld32(o_base + c * 32, r[c]);
-          tmem_ld_wait();
-          tc_fence_before_sync();
-        } else {
+        for (int c = 0; c < D / 32; ++c)
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c)
+          for (int j = 0; j < 32; ++j) r[c][j] = 0u;
+      }
 #pragma unroll
-            for (int j = 0; j < 32; ++j) r[c][j] = 0u;
-        }
-#pragma unroll
-        for (int ci = 0; ci < D / 8; ++ci) {  // 16-byte chunks of the row
-          const uint32_t* x = r[ci >> 2] + (ci & 3) * 8;
-          uint4 out;
-          out.x = DT<T>::pack(__uint_as_float(x[0]) * inv, __uint_as_float(x[1]) * inv);
-          out.y = DT<T>::pack(__uint_as_float(x[2]) * inv, __uint_as_float(x[3]) * inv);
-          out.z = DT<T>::pack(__uint_as_float(x[4]) * inv, __uint_as_float(x[5]) * inv);
-          out.w = DT<T>::pack(__uint_as_float(x[6]) * inv, __uint_as_float(x[7]) * inv);
-          if (staged) {
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(stage + (ci >> 3) * PANEL_BYTES + (((ci & 7) ^ (row & 7)) << 4)),
-                         "r"(out.x), "r"(out.y), "r"(out.z), "r"(out.w) : "memory");
-          } else if (valid) {
-            *reinterpret_cast<uint4*>(orow + ci * 8) = out;
-          }
+      for (int ci = 0; ci < D / 8; ++ci) {  // 16-byte chunks of the row
+        const uint32_t* x = r[ci >> 2] + (ci & 3) * 8;
+        uint4 out;
+        out.x = DT<T>::pack(__uint_as_float(x[0]) * inv, __uint_as_float(x[1]) * inv);
+        out.y = DT<T>::pack(__uint_as_float(x[2]) * inv, __uint_as_float(x[3]) * inv);
+        out.z = DT<T>::pack(__uint_as_float(x[4]) * inv, __uint_as_float(x[5]) * inv);
+        out.w = DT<T>::pack(__uint_as_float(x[6]) * inv, __uint_as_float(x[7]) * inv);
+        if (staged) {
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(stage + (ci >> 3) * PANEL_BYTES + (((ci & 7) ^ (row & 7)) << 4)),
+                       "r"(out.x), "r"(out.y), "r"(out.z), "r"(out.w) : "memory");
+        } else if (valid) {
+          *reinterpret_cast<uint4*>(orow + ci * 8) = out;
         }
       }
       if (ntiles > 0) {
@@ -723,22 +507,7 @@ dense_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   if (warp == kTcSoftWarps + 1) tmem_dealloc(tmem, 512);
 }
 
-// The two boxes of a split tile of K and V (none where the sinks fill whole tiles).
-int make_sink_maps(SinkMaps& m, CUtensorMapDataType dt, const void* q, const void* k, const void* v, const void* dout, const long long* S, int D,
-                   int Hkv, int Nk, int sinks, int tile) {
-  m.q = q; m.keys = k; m.values = v; m.dout = dout;
-  m.q_sn = S[0]; m.q_sh = S[1]; m.k_sn = S[2]; m.k_sh = S[3]; m.v_sn = S[4]; m.v_sh = S[5]; m.do_sn = S[6]; m.do_sh = S[7];
-  const int first = sink_room(sinks) % tile;
-  for (int x = 0; x < 2; ++x) {
-    const int rows = first == 0 ? tile : x ? tile - first : first;
-    int rc = make_tmap_3d(&m.k[x], dt, k, D, Hkv, Nk, S[3], S[2], 64, 1, rows);
-    if (!rc) rc = make_tmap_3d(&m.v[x], dt, v, D, Hkv, Nk, S[5], S[4], 64, 1, rows);
-    if (rc) return rc;
-  }
-  return kOk;
-}
-
-template <typename T, int D, bool SINKS>
+template <typename T, int D>
 static int launch_dense_fwd_tc(const void* q, const void* k, const void* v, const long long* S, int Nq, int Nk, DenseFwdTcParams p, cudaStream_t stream) {
   // S: q_n q_h k_n k_h v_n v_h o_n o_h
   CUtensorMap tmQ, tmK, tmV;
@@ -753,38 +522,28 @@ static int launch_dense_fwd_tc(const void* q, const void* k, const void* v, cons
   rc = make_tmap_3d(&tmO, DT<T>::kTmapType, p.o, D, p.Hq, Nq, p.o_sh, p.o_sn, 64, p.G, QT);
   if (rc) return rc;
   const size_t smem = (kTcQBufs + 2 * kTcStages) * 128 * D * 2 + sizeof(StealSlot) + sizeof(ItemRing) + 24 * sizeof(uint64_t);
-  TileMaps<SINKS> split;
-  if constexpr (SINKS) {
-    rc = make_sink_maps(split, DT<T>::kTmapType, q, k, v, nullptr, S, D, p.Hkv, Nk, p.sinks, kTcKeyTile);
-    if (rc) return rc;
-  }
-  auto kern = dense_fwd_tc_kernel<T, D, SINKS>;
+  auto kern = dense_fwd_tc_kernel<T, D>;
   cudaError_t e = allow_smem(kern, smem);
   if (e != cudaSuccess) return cuda_rc(e);
   const dim3 grid((unsigned)row_tile_slots(Nq, p.B, 8 - p.logG), p.Hkv);
-  { LaunchScope ls_(SINKS ? "sink_fwd_tc" : "dense_fwd_tc", stream); kern<<<grid, kTcThreads, smem, stream>>>(tmQ, tmK, tmV, tmO, p, split); }
+  { LaunchScope ls_("dense_fwd_tc", stream); kern<<<grid, kTcThreads, smem, stream>>>(tmQ, tmK, tmV, tmO, p); }
   return cuda_rc(cudaGetLastError());
 }
 
-template <typename T, int D>
-static int launch_dense(const void* q, const void* k, const void* v, const long long* S, int Nq, int Nk, DenseFwdTcParams p, cudaStream_t stream) {
-  return p.sinks < 0 ? launch_dense_fwd_tc<T, D, false>(q, k, v, S, Nq, Nk, p, stream) : launch_dense_fwd_tc<T, D, true>(q, k, v, S, Nq, Nk, p, stream);
-}
-
-// entry used by nsa_varlen_attn_fwd (dense_fwd.cu) and, with sinks >= 0, by nsa_sink_window_attn_fwd
+// entry used by nsa_varlen_attn_fwd (dense_fwd.cu)
 int varlen_attn_fwd_tc(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, void* o, float* lse,
                        int total_q, int total_k, int batch, int Hq, int Hkv, int head_dim, int causal,
-                       int window, int stride, int left, int sinks, void* rest, const long long* strides, float sm_scale, int dtype, cudaStream_t stream) {
+                       int window, int stride, int left, const long long* strides, float sm_scale, int dtype, cudaStream_t stream) {
   DenseFwdTcParams p;
   p.o = o; p.lse = lse; p.cu_q = cu_q; p.cu_k = cu_k;
   p.o_sn = strides[6]; p.o_sh = strides[7];
   p.B = batch; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
   p.logG = 0;
   while ((1 << p.logG) < p.G) ++p.logG;
-  p.window = window; p.stride = stride; p.causal = causal; p.left = left; p.sinks = sinks; p.rows = total_q; p.rest = static_cast<uint4*>(rest);
+  p.window = window; p.stride = stride; p.causal = causal; p.left = left;
   p.scale2 = sm_scale * kLog2e;
   p.st.word = status_word();
-  return NSA_DISPATCH_T_D(dtype, head_dim, launch_dense, q, k, v, strides, total_q, total_k, p, stream);
+  return NSA_DISPATCH_T_D(dtype, head_dim, launch_dense_fwd_tc, q, k, v, strides, total_q, total_k, p, stream);
 }
 
 }  // namespace nsa

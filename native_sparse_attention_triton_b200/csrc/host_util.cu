@@ -63,7 +63,7 @@ SmemGrant g_grants[kGrants];
 std::atomic<int> g_sms[64];
 }  // namespace
 
-cudaError_t allow_smem(const void* kernel, int bytes) {
+cudaError_t allow_smem(const void* kernel, int bytes, bool shared_sm) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -82,6 +82,7 @@ cudaError_t allow_smem(const void* kernel, int bytes) {
   std::lock_guard<std::mutex> lk(mu);
   if (g && g->bytes[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && shared_sm) e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
   if (e == cudaSuccess && g) g->bytes[dev].store(bytes, std::memory_order_release);
   return e;
 }

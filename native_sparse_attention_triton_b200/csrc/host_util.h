@@ -29,11 +29,12 @@ int make_tmap_4d(CUtensorMap* out, CUtensorMapDataType dt, const void* base, uin
                  uint32_t b3 = 1);
 
 // Opt `kernel` in to `bytes` of dynamic shared memory on the current device.  The runtime call costs about a microsecond of
-// host time, so what has been granted is remembered per (kernel, device) and asked for once.
-cudaError_t allow_smem(const void* kernel, int bytes);
+// host time, so what has been granted is remembered per (kernel, device) and asked for once.  `shared_sm`: CTAs of it are to share an SM, whose
+// first-level cache then leaves as much to shared memory as it can.
+cudaError_t allow_smem(const void* kernel, int bytes, bool shared_sm = false);
 template <typename K>
-cudaError_t allow_smem(K* kernel, size_t bytes) {
-  return allow_smem(reinterpret_cast<const void*>(kernel), static_cast<int>(bytes));
+cudaError_t allow_smem(K* kernel, size_t bytes, bool shared_sm = false) {
+  return allow_smem(reinterpret_cast<const void*>(kernel), static_cast<int>(bytes), shared_sm);
 }
 
 // multiprocessors of the current device (remembered)

@@ -364,7 +364,7 @@ static int launch_sink_dq(const void* k, const void* v, const long long* S, int 
   p.rows = total;
   const size_t smem = (size_t)(2 * 128 + (kKStages + 1) * kKeys) * D * 2 + 128 * sizeof(float) + 16 * sizeof(uint64_t) + 16;
   auto kern = sink_dq_tc_kernel<T, D>;
-  cudaError_t e = allow_smem(kern, smem);
+  cudaError_t e = allow_smem(kern, smem, /*shared_sm=*/true);
   if (e != cudaSuccess) return cuda_rc(e);
   const dim3 grid((unsigned)row_tile_slots(total, p.B, 7 - p.logG), p.Hkv);
   { LaunchScope ls_("sink_dq_tc", stream); kern<<<grid, 320, smem, stream>>>(tmQ, tmDO, tmK, tmV, tmDQ, p, split); }

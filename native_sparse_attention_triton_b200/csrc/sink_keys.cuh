@@ -1,15 +1,13 @@
 // The keys that rows of a sliding window with sinks see, without the gap between the two.
 //
 // Query t of a sequence sees key j <= t iff t - j <= left or j < sinks.  A group of rows at tokens q0, q0 + 1, ... takes its keys in tiles
-// (128 forward, 64 backward) from the list
+// from the list
 //     column u:  key u                for u < room,      room = sinks rounded up to 8 rows (the swizzle's unit),
 //                key u + shift        for u >= room,     shift = max(0, q0 - left - room),
 // so the window starts at the first key that any of the rows sees, wherever that lies, and the sinks fill the head of the first tile
 // instead of costing a tile of their own.  The tile in which the list jumps is loaded by two TMA boxes.  Columns [sinks, room) are hidden from
 // every row where there is a gap (their keys lie in front of the window), and are ordinary keys where there is none.
 #pragma once
-#include <type_traits>
-
 #include "tc5.cuh"
 
 namespace nsa {
@@ -21,9 +19,6 @@ struct SinkMaps {
   const void *q, *keys, *values, *dout;
   long long q_sn, q_sh, k_sn, k_sh, v_sn, v_sh, do_sn, do_sh;
 };
-struct NoMaps {};
-template <bool SINKS>
-using TileMaps = std::conditional_t<SINKS, SinkMaps, NoMaps>;
 
 __host__ __device__ __forceinline__ int sink_room(int sinks) { return (sinks + 7) & ~7; }
 __device__ __forceinline__ int sink_shift(int q0, int left, int room) { return max(0, q0 - left - room); }

@@ -823,24 +823,56 @@ static int run_dense_bwd(const void* q, const void* k, const void* v, const void
   return cv.run<T>(stream);
 }
 
-// Tokens per CTA of the dK/dV pass of a window with sinks, in row tiles of 128 / G tokens: all that see a key tile where that leaves two
-// CTAs for every SM.
+// Tokens per CTA of the dK/dV pass of a window with sinks, in row tiles of 128 / G tokens: all that see a key tile, up to 160 tiles, where that
+// leaves two CTAs for every SM (then dK and dV need no fp32 sums, which cost 32 768 tokens 64q/4kv 65 us and a memset); else up to 64.
 static int sink_chunk(int total, int batch, int Hkv, int G, int left) {
   const int per = 128 / G;
   const long long tiles = (total / 128ll + batch) * Hkv;
-  const int span = std::min<long long>(total, (long long)left + 128);
-  int chunk = std::min(64, (span + per - 1) / per);
+  const int span = (int)std::min<long long>(total, (long long)left + 128), all = (span + per - 1) / per;
+  int chunk = all <= 160 ? all : 64;
   while (chunk > 4 && tiles * ((span + chunk * per - 1) / (chunk * per)) < 2 * 148) chunk = (chunk + 1) / 2;
   return chunk * per;
 }
 
+// Which rows of dK and dV are summed up in fp32: all of them, or (where a CTA of the dK/dV pass has all of a key tile's tokens) those of the
+// tiles that hold a sequence's sinks, `tiles` of them.  Row x of the grid's; false where it stands for none.
+struct SummedRows {
+  const int* cu;
+  int B, tiles, total;  // tiles < 0: all
+  __host__ __device__ long long count() const { return tiles < 0 ? total : (long long)B * tiles * 128; }
+  __device__ __forceinline__ bool row(long long x, int& n) const {
+    if (tiles < 0) {
+      n = (int)x;
+      return true;
+    }
+    const int b = (int)(x / (tiles * 128)), at = (int)(x % (tiles * 128)), start = __ldg(cu + b);
+    n = start + at;
+    return at < __ldg(cu + b + 1) - start;
+  }
+};
+
+// A warp per row of a head.
+template <int D>
+__global__ void __launch_bounds__(256) sink_zero_kernel(SummedRows r, float* dk32, float* dv32, int Hkv) {
+  const long long x = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  int n;
+  if (x >= r.count() * Hkv || !r.row(x / Hkv, n)) return;
+  const long long at = ((long long)n * Hkv + x % Hkv) * D;
+  for (int c = lane_id() * 4; c < D; c += 128) {
+    *reinterpret_cast<float4*>(dk32 + at + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+    *reinterpret_cast<float4*>(dv32 + at + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+}
+
 // fp32 sums of dK and dV -> storage type; a warp per row of a head.  Rows with a value that is not finite are computed one by one.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) sink_finish_kernel(DkdvParams p, const __grid_constant__ SinkMaps maps, void* dk, void* dv, long long dk_sn,
-                                                          long long dk_sh, long long dv_sn, long long dv_sh, int rows) {
-  const long long x = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (x >= (long long)rows * p.Hkv) return;
-  const int n = (int)(x / p.Hkv), h = (int)(x % p.Hkv), lane = lane_id();
+__global__ void __launch_bounds__(256) sink_finish_kernel(DkdvParams p, SummedRows r, const __grid_constant__ SinkMaps maps, void* dk, void* dv,
+                                                          long long dk_sn, long long dk_sh, long long dv_sn, long long dv_sh) {
+  long long x = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  int n;
+  if (x >= r.count() * p.Hkv || !r.row(x / p.Hkv, n)) return;
+  const int h = (int)(x % p.Hkv), lane = lane_id();
+  x = (long long)n * p.Hkv + h;
   float4 a, b;
   if constexpr (D == 128) {
     a = __ldcs(reinterpret_cast<const float4*>(p.dk32 + x * D) + lane);
@@ -850,9 +882,8 @@ __global__ void __launch_bounds__(256) sink_finish_kernel(DkdvParams p, const __
     a = make_float4(a2.x, a2.y, 0.f, 0.f);
     b = make_float4(b2.x, b2.y, 0.f, 0.f);
   }
-  const float top = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))), fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w))));
-  const bool nan = a.x != a.x || a.y != a.y || a.z != a.z || a.w != a.w || b.x != b.x || b.y != b.y || b.z != b.z || b.w != b.w;
-  if (__any_sync(0xffffffffu, nan || top == INFINITY) && n < __ldg(p.cu_q + p.B)) {
+  const float zero = (a.x + a.y + a.z + a.w) * 0.f + (b.x + b.y + b.z + b.w) * 0.f;
+  if (__any_sync(0xffffffffu, zero != 0.f) && n < __ldg(p.cu_q + p.B)) {
     const int s = find_sequence(p.cu_q, p.B, n), row0 = __ldg(p.cu_q + s);
     exact_key_row<T, D>(a, b, &maps, p.ld, p.Hq, row0, __ldg(p.cu_q + s + 1) - row0, n - row0, h, p.G, p.left, p.sinks, p.scale2, p.sm_scale);
   }
@@ -872,8 +903,6 @@ static int run_sink_bwd(const void* q, const void* k, const void* v, const void*
   w += align_up((size_t)total * Hkv * D * sizeof(float), 256);
   float* dv32 = reinterpret_cast<float*>(w);
   w += align_up((size_t)total * Hkv * D * sizeof(float), 256);
-  cudaError_t e = cudaMemsetAsync(dk32, 0, w - reinterpret_cast<uint8_t*>(dk32), stream);
-  if (e != cudaSuccess) return cuda_rc(e);
   DenseBwdParams p;
   p.q = q; p.o = o; p.dout = dout; p.lse = lse; p.ld = ld; p.dq = dq; p.cu_q = cu; p.cu_k = cu;
   p.q_sn = S[0]; p.q_sh = S[1]; p.o_sn = S[6]; p.o_sh = S[7]; p.do_sn = S[8]; p.do_sh = S[9]; p.dq_sn = S[10]; p.dq_sh = S[11];
@@ -897,13 +926,22 @@ static int run_sink_bwd(const void* q, const void* k, const void* v, const void*
   d.key_slots = (int)row_tile_slots(total, batch, 7);
   d.sink_log = 13 - p.logG;  // 64 row tiles
   while (d.sink_log > 9 - p.logG && row_tile_slots(total, batch, d.sink_log) * Hkv < 148) --d.sink_log;
-  rc = launch_dense_dkdv_tc<T, D>(q, dout, k, v, ds, total, total, (int)std::min<long long>(total, (long long)left + 128), 0, batch, d, stream);
-  if (rc) return rc;
+  const int span = (int)std::min<long long>(total, (long long)left + 128);
+  const SummedRows summed{cu, batch, span > d.chunk ? -1 : (sinks + 127) / 128, total};
+  const long long warps = summed.count() * Hkv;
+  if (summed.tiles < 0) {
+    cudaError_t e = cudaMemsetAsync(dk32, 0, w - reinterpret_cast<uint8_t*>(dk32), stream);
+    if (e != cudaSuccess) return cuda_rc(e);
+  } else if (warps > 0) {
+    LaunchScope ls_("sink_zero", stream);
+    sink_zero_kernel<D><<<(unsigned)((warps + 7) / 8), 256, 0, stream>>>(summed, dk32, dv32, Hkv);
+  }
+  rc = launch_sink_dkdv_tc<T, D>(q, dout, k, v, dk, dv, ds, S + 12, total, span, d, stream);
+  if (rc || warps == 0) return rc;
   SinkMaps maps;
-  rc = make_sink_maps(maps, DT<T>::kTmapType, q, k, v, dout, ds, D, Hkv, total, sinks, 128);
-  if (rc) return rc;
+  sink_inputs(maps, q, k, v, dout, ds);
   LaunchScope ls_("sink_finish", stream);
-  sink_finish_kernel<T, D><<<(unsigned)(((long long)total * Hkv + 7) / 8), 256, 0, stream>>>(d, maps, dk, dv, S[12], S[13], S[14], S[15], total);
+  sink_finish_kernel<T, D><<<(unsigned)((warps + 7) / 8), 256, 0, stream>>>(d, summed, maps, dk, dv, S[12], S[13], S[14], S[15]);
   return cuda_rc(cudaGetLastError());
 }
 

@@ -97,6 +97,13 @@ template <typename T, int D>
 int launch_dense_dkdv_tc(const void* q, const void* dout, const void* k, const void* v, const long long* strides, int Nq, int Nk,
                          int max_q, int max_k, int batch, DkdvParams p, cudaStream_t stream);
 
+// dK/dV pass of the sliding window with sinks (sink_dkdv_tc.cu); S: q_n q_h k_n k_h v_n v_h do_n do_h, G: dk_n dk_h dv_n dv_h; span: the most
+// tokens a key tile's window reaches.  With span <= p.chunk it writes dK and dV of key tiles without sinks itself, else all of them go
+// into p.dk32 and p.dv32 (zeroed).
+template <typename T, int D>
+int launch_sink_dkdv_tc(const void* q, const void* dout, const void* k, const void* v, void* dk, void* dv, const long long* S, const long long* G,
+                        int total, int span, DkdvParams p, cudaStream_t stream);
+
 // dQ, dK and dV of the dense attention in one pass (dense_bwd_tc.cu); head_dim 128, group size a power of two <= 16.
 // p.chunk = tokens per CTA; p.dq32 zeroed like p.dk32 and p.dv32.  No sliding window: p.left is not read.
 template <typename T>

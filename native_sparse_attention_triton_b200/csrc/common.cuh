@@ -144,6 +144,9 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return d;
 }
 
+// In a kernel that was launched early (host_util.h): the kernel in front of it has finished and its writes are visible.
+__device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+
 __device__ __forceinline__ int lane_id() { return threadIdx.x & 31; }
 
 // largest b such that cu[b] <= n (cu has nseq+1 ascending entries, cu[0] = 0)

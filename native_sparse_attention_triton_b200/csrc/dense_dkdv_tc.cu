@@ -20,7 +20,6 @@
 // TMEM columns: dV [0,128)  dK [128,256)  S^T / P^T [256,384)  dP^T / dS^T [384,512).
 #include "dense_bwd_tile.cuh"
 #include "host_util.h"
-#include "work_steal.cuh"
 
 namespace nsa {
 namespace {
@@ -29,9 +28,7 @@ constexpr int kDoStages = 2;
 constexpr int kPanelBytes = 128 * 128;  // [128][64] 16-bit elements; an operand tile of 128 x D is D / 64 of them
 }  // namespace
 
-// SINKS: a sliding window with sinks.  A CTA does either a key tile and a part of the tokens whose window it lies in, or (for the sinks of a
-// sequence) a tile of sinks and a part of the tokens past their window; both add to the same sums.  Its sequence is searched for.
-template <typename T, int D, bool SINKS>
+template <typename T, int D>
 __global__ void __launch_bounds__(320, 1)
 dense_dkdv_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
                      const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, DkdvParams p, int logG) {
@@ -69,47 +66,20 @@ dense_dkdv_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   }
 
   // ---- which key tile, which tokens ----
-  int b, h, qs, Lq, kpos, krow0, kvalid, tok_begin, tok_end;
-  bool far = false;  // sinks and the tokens past their window
-  if constexpr (SINKS) {
-    h = blockIdx.z;
-    int slot = blockIdx.x, tile, st = 0;
-    far = slot >= p.key_slots;
-    if (far) {
-      if (blockIdx.y > 0) return;
-      const int st_tiles = (p.sinks + KT - 1) / KT;
-      slot -= p.key_slots;
-      st = slot % st_tiles;
-      slot /= st_tiles;
-    }
-    if (!find_row_tile(p.cu_q, p.B, far ? p.sink_log : 7, slot, b, qs, Lq, tile)) return;
-    kpos = (far ? st : tile) * KT;
-    krow0 = qs + kpos;
-    kvalid = min(KT, (far ? min(p.sinks, Lq) : Lq) - kpos);
-    if (far) {
-      tok_begin = max(tile << p.sink_log, kpos + p.left + 1);
-      tok_end = min((tile + 1) << p.sink_log, Lq);
-      if (kvalid <= 0) return;
-    } else {
-      tok_begin = kpos + blockIdx.y * p.chunk;
-      tok_end = min(min(tok_begin + p.chunk, Lq), kpos + kvalid + p.left);
-    }
-  } else {
-    b = blockIdx.z / p.Hkv;
-    h = blockIdx.z % p.Hkv;
-    qs = __ldg(p.cu_q + b);
-    Lq = __ldg(p.cu_q + b + 1) - qs;
-    const int ks0 = __ldg(p.cu_k + b), Lk = __ldg(p.cu_k + b + 1) - ks0;
-    kpos = blockIdx.x * KT;  // key tiles vary fastest: CTAs that run together share a token chunk in L2
-    if (kpos >= Lk) return;
-    krow0 = ks0 + kpos;
-    kvalid = min(KT, Lk - kpos);
-    const int t_first = p.causal ? kpos * p.stride + p.window - 1 : 0;
-    const int c_lo = blockIdx.y * p.chunk;
-    tok_begin = max(c_lo, t_first);
-    // sliding window: key j is seen by tokens up to j + left only
-    tok_end = p.left >= 0 ? min(min(c_lo + p.chunk, Lq), kpos + kvalid + p.left) : min(c_lo + p.chunk, Lq);
-  }
+  const int b = blockIdx.z / p.Hkv;
+  const int h = blockIdx.z % p.Hkv;
+  const int qs = __ldg(p.cu_q + b);
+  const int Lq = __ldg(p.cu_q + b + 1) - qs;
+  const int ks0 = __ldg(p.cu_k + b), Lk = __ldg(p.cu_k + b + 1) - ks0;
+  const int kpos = blockIdx.x * KT;  // key tiles vary fastest: CTAs that run together share a token chunk in L2
+  if (kpos >= Lk) return;
+  const int krow0 = ks0 + kpos;
+  const int kvalid = min(KT, Lk - kpos);
+  const int t_first = p.causal ? kpos * p.stride + p.window - 1 : 0;
+  const int c_lo = blockIdx.y * p.chunk;
+  const int tok_begin = max(c_lo, t_first);
+  // sliding window: key j is seen by tokens up to j + left only
+  const int tok_end = p.left >= 0 ? min(min(c_lo + p.chunk, Lq), kpos + kvalid + p.left) : min(c_lo + p.chunk, Lq);
   if (tok_end <= tok_begin) return;
   const int ntiles = (tok_end - tok_begin + TPT - 1) / TPT;
 
@@ -216,10 +186,6 @@ dense_dkdv_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           progressed = true;
         }
         if (ns < ntiles && ns == nv && mbar_test(q_full + (ns % kQStages), (ns / kQStages) & 1)) {
-          if constexpr (SINKS) {
-            if (ns == ntiles - 1 && tok_begin + ntiles * TPT > tok_end)
-              zero_tile_rows<PANELS, kPanelBytes>(q_base + (ns % kQStages) * TILE_BYTES, (tok_end - tok_begin - ns * TPT) << logG, 128);
-          }
           tc_fence_after_sync();
           issue_logits(k_addr, q_base + (ns % kQStages) * TILE_BYTES, tmem + 256, s_full);
           ++ns;
@@ -232,10 +198,6 @@ dense_dkdv_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           progressed = true;
         }
         if (np < ntiles && np == nk && mbar_test(do_full + (np % kDoStages), (np / kDoStages) & 1)) {
-          if constexpr (SINKS) {
-            if (np == ntiles - 1 && tok_begin + ntiles * TPT > tok_end)
-              zero_tile_rows<PANELS, kPanelBytes>(do_base + (np % kDoStages) * TILE_BYTES, (tok_end - tok_begin - np * TPT) << logG, 128);
-          }
           tc_fence_after_sync();
           issue_logits(v_addr, do_base + (np % kDoStages) * TILE_BYTES, tmem + 384, dp_full);
           ++np;
@@ -262,7 +224,7 @@ dense_dkdv_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const int key = (warp & 3) * 32 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     // first in-sequence token position that sees this key
-    const int thr = SINKS ? kpos + key + (far ? p.left + 1 : 0) : p.causal ? (kpos + key) * p.stride + p.window - 1 : 0;
+    const int thr = p.causal ? (kpos + key) * p.stride + p.window - 1 : 0;
     const bool key_ok = key < kvalid;
     for (int i = 0; i < ntiles; ++i) {
       const int ms = i & 1;
@@ -270,7 +232,7 @@ dense_dkdv_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       // visible columns of this thread: [clo, chi) in tile columns, shifted to the thread's own 64
       const int clo = max(0, thr - tok0) << logG;
       int chi = key_ok ? (min(TPT, tok_end - tok0) << logG) : 0;
-      if (SINKS ? !far : p.left >= 0) chi = min(chi, max(0, kpos + key + p.left - tok0 + 1) << logG);
+      if (p.left >= 0) chi = min(chi, max(0, kpos + key + p.left - tok0 + 1) << logG);
       const int clo_rel = clo - half * 64;
       const unsigned span = chi > clo ? (unsigned)(chi - clo) : 0u;
 
@@ -278,13 +240,7 @@ dense_dkdv_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       mbar_wait(s_full, i & 1, p.st);
       tc_fence_after_sync();
       float pf[64];
-      // a row tile that no key of the warp is seen by: at the edges of a window that is every other one
-      const bool none = SINKS && __all_sync(0xffffffffu, span == 0u);
-      if (none) {
-        const uint32_t zero[32] = {};
-        tmem_st32(lane_base + 256 + half * 64, zero);
-        tmem_st_wait();
-      } else {
+      {
         uint32_t su[2][32];
         tmem_ld32(lane_base + 256 + half * 64, su[0]);
         tmem_ld32(lane_base + 256 + half * 64 + 32, su[1]);
@@ -302,11 +258,7 @@ dense_dkdv_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 
       mbar_wait(dp_full, i & 1, p.st);
       tc_fence_after_sync();
-      if (none) {
-        const uint32_t zero[32] = {};
-        tmem_st32(lane_base + 384 + half * 64, zero);
-        tmem_st_wait();
-      } else {
+      {
         uint32_t du[2][32];
         tmem_ld32(lane_base + 384 + half * 64, du[0]);
         tmem_ld32(lane_base + 384 + half * 64 + 32, du[1]);
@@ -333,8 +285,8 @@ dense_dkdv_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
-template <typename T, int D, bool SINKS>
-static int launch_dkdv_tc(const void* q, const void* dout, const void* k, const void* v, const long long* strides, int Nq, int Nk,
+template <typename T, int D>
+int launch_dense_dkdv_tc(const void* q, const void* dout, const void* k, const void* v, const long long* strides, int Nq, int Nk,
                          int max_q, int max_k, int batch, DkdvParams p, cudaStream_t stream) {
   constexpr int TILE_BYTES = D / 64 * kPanelBytes;
   int logG = 0;
@@ -350,23 +302,12 @@ static int launch_dkdv_tc(const void* q, const void* dout, const void* k, const 
   rc = make_tmap_3d(&tmV, DT<T>::kTmapType, v, D, p.Hkv, Nk, strides[5], strides[4], 64, 1, 128);
   if (rc) return rc;
   const size_t smem = (size_t)(2 + kQStages + kDoStages) * TILE_BYTES + 4 * 128 * sizeof(float) + 24 * sizeof(uint64_t) + 16;
-  auto kern = dense_dkdv_tc_kernel<T, D, SINKS>;
+  auto kern = dense_dkdv_tc_kernel<T, D>;
   cudaError_t e = allow_smem(kern, smem);
   if (e != cudaSuccess) return cuda_rc(e);
   dim3 grid((max_k + 127) / 128, (max_q + p.chunk - 1) / p.chunk, batch * p.Hkv);
-  if (SINKS) {  // max_q stands for the tokens that see a key tile's window
-    const long long far = p.sinks > 0 ? row_tile_slots(Nq, p.B, p.sink_log) * ((p.sinks + 127) / 128) : 0;
-    grid = dim3((unsigned)(p.key_slots + far), (max_q + p.chunk - 1) / p.chunk, p.Hkv);
-  }
-  { LaunchScope ls_(SINKS ? "sink_dkdv_tc" : "dense_dkdv_tc", stream); kern<<<grid, 320, smem, stream>>>(tmQ, tmDO, tmK, tmV, p, logG); }
+  { LaunchScope ls_("dense_dkdv_tc", stream); kern<<<grid, 320, smem, stream>>>(tmQ, tmDO, tmK, tmV, p, logG); }
   return cuda_rc(cudaGetLastError());
-}
-
-template <typename T, int D>
-int launch_dense_dkdv_tc(const void* q, const void* dout, const void* k, const void* v, const long long* strides, int Nq, int Nk, int max_q, int max_k,
-                         int batch, DkdvParams p, cudaStream_t stream) {
-  return p.sinks < 0 ? launch_dkdv_tc<T, D, false>(q, dout, k, v, strides, Nq, Nk, max_q, max_k, batch, p, stream)
-                     : launch_dkdv_tc<T, D, true>(q, dout, k, v, strides, Nq, Nk, max_q, max_k, batch, p, stream);
 }
 
 #define NSA_INSTANTIATE(T, D)                                                                                                         \

@@ -7,7 +7,7 @@
 // Eviction, for every (sequence, KV head) with L > budget rows: kept are the first `sinks` rows, the last `recent` ones, and of those
 // between the r = budget - sinks - recent with the largest weights, equal ones by the lower row; a weight that is no number counts as
 // the smallest.  The kept rows go, in their order, to the first `budget` rows of other pages.  `evict_select` finds the r-th largest
-// weight by a radix selection on the bits of the weights, eight at a time, then numbers the kept rows; `evict_move` copies them.
+// weight by a radix selection on the bits of the weights, eleven at a time, then numbers the kept rows; `evict_move` copies them.
 #include "dispatch.h"
 #include "host_util.h"
 #include "nsa_b200.h"
@@ -91,6 +91,8 @@ struct PagedEvictParams {
 };
 
 constexpr int kSelectThreads = 512;
+constexpr int kSelectItems = 16;  // rows a thread holds in registers
+constexpr int kBins = 2048;
 
 // Larger weights have larger keys; both zeros the same one.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -99,8 +101,8 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Exclusive sum over the block's threads of two counts below 65536 each, packed in one word; `total` gets the sum of all.
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, uint32_t& total) {
+// Exclusive sum over the block's threads; `total` gets the sum of all.  `sums`: a word a warp, free again after the next barrier.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* sums, uint32_t& total) {
   const int lane = lane_id(), warp = threadIdx.x >> 5;
   uint32_t up = v;
 #pragma unroll
@@ -108,23 +110,26 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, 
     const uint32_t y = __shfl_up_sync(0xffffffffu, up, s);
     if (lane >= s) up += y;
   }
-  __syncthreads();
-  if (lane == 31) warp_sums[warp] = up;
+  if (lane == 31) sums[warp] = up;
   __syncthreads();
   uint32_t before = 0;
   total = 0;
 #pragma unroll
   for (int w = 0; w < kSelectThreads / 32; ++w) {
-    const uint32_t x = warp_sums[w];
+    const uint32_t x = sums[w];
     before += w < warp ? x : 0;
     total += x;
   }
   return before + up - v;
 }
 
+// A CTA per (sequence, KV head).  A warp holds neighbouring rows, 32 at a time, so that votes and one scan over the warps number them and what is
+// written lies together; up to 8192 rows stay in registers, longer sequences are read again for every pass, 8192 rows at a time.  Digits of
+// 11, 11 and 10 bits: the first (sign, exponent and two bits) spreads weights over enough bins that the atomics on shared memory do not queue.
+// What bounds it is the chain of its passes.
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(PagedEvictParams p) {
-  __shared__ unsigned hist[256];
-  __shared__ uint32_t warp_sums[kSelectThreads / 32];
+  __shared__ unsigned hist[kBins];
+  __shared__ uint32_t sums[4][kSelectThreads / 32];
   __shared__ uint32_t s_digit, s_rank;
   const int b = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv, tid = threadIdx.x;
   const int len = __ldg(p.seqlens + b), L = max(0, min(len, p.cap)), m = min(L, p.budget);
@@ -142,72 +147,100 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(PagedEvict
     }
     return;
   }
-  // ---- the key of the r-th largest weight between the sinks and the recent rows, and how many of its equals are kept ----
+  // this thread's rows of a span: base + first + 32 j for j < per
+  constexpr int kSpan = kSelectThreads * kSelectItems;
+  const int per = min(kSelectItems, (L + kSelectThreads - 1) / kSelectThreads), span = per * kSelectThreads;
+  const int lane = lane_id(), warp = tid >> 5, first = warp * per * 32 + lane;
   const int lo = p.sinks, hi = L - p.recent;
+  float x[kSelectItems];
+  uint32_t within, between;  // which of them are rows, and which of those are neither sinks nor recent
+  auto load = [&](int base) {
+    within = between = 0;
+#pragma unroll
+    for (int j = 0; j < kSelectItems; ++j) {
+      const int i = base + first + 32 * j;
+      const bool in = j < per && i < L;
+      x[j] = in ? __ldg(w + i) : 0.f;
+      within |= (in ? 1u : 0u) << j;
+      between |= (in && i >= lo && i < hi ? 1u : 0u) << j;
+    }
+  };
+  load(0);
+  // ---- the key of the r-th largest weight between the sinks and the recent rows, and how many of its equals are kept ----
   int rank = p.budget - p.sinks - p.recent;  // below the number of rows between
-  uint32_t found = 0, mask = 0;
+  uint32_t found = 0xffffffffu;              // above every key
   if (rank > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kSelectThreads) hist[i] = 0;
+    found = 0;
+    uint32_t mask = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      const uint32_t digit = pass == 2 ? 1023u : 2047u;
+      for (int i = tid; i < kBins; i += kSelectThreads) hist[i] = 0;
       __syncthreads();
-      for (int i = lo + tid; i < hi; i += kSelectThreads) {
-        const uint32_t key = weight_key(__ldg(w + i));
-        if ((key & mask) == found) atomicAdd(hist + (key >> shift & 255u), 1u);
+      for (int base = 0; base < L; base += span) {
+        if (L > kSpan) load(base);
+#pragma unroll
+        for (int j = 0; j < kSelectItems; ++j) {
+          if (j >= per) break;
+          const uint32_t key = weight_key(x[j]);
+          if ((between >> j & 1u) && (key & mask) == found) atomicAdd(hist + (key >> shift & digit), 1u);
+        }
       }
       __syncthreads();
-      if (tid < 32) {  // the digit at which the counts from the top pass the rank; eight digits a lane, the largest first
-        unsigned own = 0;
+      // the digit at which the counts from the top pass the rank; a thread has four neighbouring ones, the largest first
+      uint32_t own = 0, total;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) own += hist[255 - tid * 8 - x];
-        unsigned upto = own;
-#pragma unroll
-        for (int s = 1; s < 32; s <<= 1) {
-          const unsigned y = __shfl_up_sync(0xffffffffu, upto, s);
-          if (tid >= s) upto += y;
-        }
-        const unsigned before = upto - own;
-        if (before < (unsigned)rank && upto >= (unsigned)rank) {
-          unsigned left = rank - before;
-          int x = 0;
-          while (hist[255 - tid * 8 - x] < left) left -= hist[255 - tid * 8 - x++];
-          s_digit = 255 - tid * 8 - x;
-          s_rank = left;
-        }
+      for (int y = 0; y < kBins / kSelectThreads; ++y) own += hist[kBins - 1 - tid * (kBins / kSelectThreads) - y];
+      const uint32_t front = block_scan(own, sums[pass], total);
+      if (front < (uint32_t)rank && front + own >= (uint32_t)rank) {
+        uint32_t left = rank - front;
+        int at = kBins - 1 - tid * (kBins / kSelectThreads);
+        while (hist[at] < left) left -= hist[at--];
+        s_digit = at;
+        s_rank = left;
       }
       __syncthreads();
       found |= s_digit << shift;
-      mask |= 255u << shift;
+      mask |= digit << shift;
       rank = s_rank;
-      __syncthreads();
     }
-  } else {
-    found = 0xffffffffu;  // above every key
   }
-  // ---- the kept rows in their order ----
+  // ---- the kept rows in their order: the sure ones, and of the last key's equals those within the rank ----
   int taken = 0, equals = 0;
-  for (int i0 = 0; i0 < L; i0 += kSelectThreads) {
-    const int i = i0 + tid;
-    float x = 0.f;
-    bool sure = false, equal = false;
-    if (i < L) {
-      x = __ldg(w + i);
-      const bool between = i >= lo && i < hi;
-      const uint32_t key = weight_key(x);
-      sure = !between || key > found;
-      equal = between && key == found && rank > 0;
+  for (int base = 0; base < L; base += span) {
+    if (L > kSpan) load(base);
+    uint32_t sure = 0, equal = 0;
+#pragma unroll
+    for (int j = 0; j < kSelectItems; ++j) {
+      const uint32_t key = weight_key(x[j]), bit = 1u << j;
+      if ((within & bit) && (!(between & bit) || key > found)) sure |= bit;
+      if ((between & bit) && key == found && rank > 0) equal |= bit;
     }
-    uint32_t all;
-    const uint32_t at = block_scan((sure ? 1u : 0u) | (equal ? 0x10000u : 0u), warp_sums, all);
-    const int eq = equals + (int)(at >> 16);
-    const bool keep = sure || (equal && eq < rank);
-    // rows kept before this one: the sure ones, and of its equals those that are still within the rank
-    const int to = taken + (int)(at & 0xffffu) + min(eq, rank) - min(equals, rank);
-    if (keep) {
-      kept[to] = i;
-      w_out[to] = x;
+    // of the warps in front: sure ones, and equals in the upper half (at most 8192 each)
+    uint32_t total;
+    const uint32_t counts = __reduce_add_sync(0xffffffffu, __popc(sure) | __popc(equal) << 16);
+    const uint32_t front = __shfl_sync(0xffffffffu, block_scan(lane == 0 ? counts : 0u, sums[3], total), 0);
+    int eq = equals + (int)(front >> 16);
+    int to = taken + (int)(front & 0xffffu) + min(eq, rank) - min(equals, rank);
+    const uint32_t below = (1u << lane) - 1u;
+#pragma unroll
+    for (int j = 0; j < kSelectItems; ++j) {
+      if (j >= per) break;
+      const uint32_t eqs = __ballot_sync(0xffffffffu, equal >> j & 1u);
+      const bool keep = (sure >> j & 1u) || ((equal >> j & 1u) && eq + __popc(eqs & below) < rank);
+      const uint32_t keeps = __ballot_sync(0xffffffffu, keep);
+      if (keep) {
+        const int at = to + __popc(keeps & below);
+        kept[at] = base + first + 32 * j;
+        w_out[at] = x[j];
+      }
+      eq += __popc(eqs);
+      to += __popc(keeps);
     }
-    taken += (int)(all & 0xffffu) + min(equals + (int)(all >> 16), rank) - min(equals, rank);
-    equals += (int)(all >> 16);
+    taken += (int)(total & 0xffffu) + min(equals + (int)(total >> 16), rank) - min(equals, rank);
+    equals += (int)(total >> 16);
+    __syncthreads();
   }
 }
 
@@ -215,6 +248,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(PagedEvict
 template <int D>
 __global__ void __launch_bounds__(256) evict_move_kernel(PagedEvictParams p) {
   constexpr int CH = D / 8, AT_ONCE = 32 / (2 * CH);  // rows copied by one step
+  wait_for_launch_before();
   const int b = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv, lane = lane_id();
   const int m = min(max(0, min(__ldg(p.seqlens + b), p.cap)), p.budget);
   const int i0 = (blockIdx.y * 8 + (threadIdx.x >> 5)) * 16;
@@ -319,10 +353,6 @@ extern "C" int nsa_paged_kv_evict(void* k_pages, void* v_pages, const int* block
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_rc(e);
   const dim3 grid(batch * num_kv_heads, (unsigned)((most + 127) / 128));
-  {
-    LaunchScope ls_("evict_move", s);
-    if (head_dim == 128) evict_move_kernel<128><<<grid, 256, 0, s>>>(p);
-    else evict_move_kernel<64><<<grid, 256, 0, s>>>(p);
-  }
-  return cuda_rc(cudaGetLastError());
+  LaunchScope ls_("evict_move", s);
+  return cuda_rc(launch_early(head_dim == 128 ? evict_move_kernel<128> : evict_move_kernel<64>, grid, 256, 0, s, p));
 }

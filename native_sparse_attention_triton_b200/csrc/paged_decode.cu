@@ -606,6 +606,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 
 // weights[b][h][j] += sum over the G heads of 2^(x_j - lse), row by row of the logits the attention kernel left.
 __global__ void __launch_bounds__(256) paged_weights_kernel(PagedDecodeParams p, float* weights, long long w_sb, long long w_sh) {
+  wait_for_launch_before();
   const int b = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv;
   const Rows rows = visible_rows(p, b);
   const int j = blockIdx.y * 256 + threadIdx.x;
@@ -645,11 +646,8 @@ static int launch_paged_decode(PagedDecodeParams p, float* weights, long long w_
   { LaunchScope ls_("paged_decode", stream); kern<<<grid, WARPS * 32, smem, stream>>>(tmK, tmV, p); }
   e = cudaGetLastError();
   if (e != cudaSuccess || !weights) return cuda_rc(e);
-  {
-    LaunchScope ls_("paged_weights", stream);
-    paged_weights_kernel<<<dim3(p.B * p.Hkv, (p.cap + 255) / 256), 256, 0, stream>>>(p, weights, w_sb, w_sh);
-  }
-  return cuda_rc(cudaGetLastError());
+  LaunchScope ls_("paged_weights", stream);
+  return cuda_rc(launch_early(paged_weights_kernel, dim3(p.B * p.Hkv, (p.cap + 255) / 256), 256, 0, stream, p, weights, w_sb, w_sh));
 }
 
 }  // namespace nsa

@@ -343,8 +343,7 @@ sink_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 
 int make_sink_maps(SinkMaps& m, CUtensorMapDataType dt, const void* q, const void* k, const void* v, const void* dout, const long long* S, int D,
                    int Hkv, int rows, int sinks, int tile) {
-  m.q = q; m.keys = k; m.values = v; m.dout = dout;
-  m.q_sn = S[0]; m.q_sh = S[1]; m.k_sn = S[2]; m.k_sh = S[3]; m.v_sn = S[4]; m.v_sh = S[5]; m.do_sn = S[6]; m.do_sh = S[7];
+  sink_inputs(m, q, k, v, dout, S);
   const int first = sink_room(sinks) % tile;
   for (int x = 0; x < 2; ++x) {
     const int height = first == 0 ? tile : x ? tile - first : first;

@@ -20,6 +20,11 @@ struct SinkMaps {
   long long q_sn, q_sh, k_sn, k_sh, v_sn, v_sh, do_sn, do_sh;
 };
 
+inline void sink_inputs(SinkMaps& m, const void* q, const void* k, const void* v, const void* dout, const long long* S) {
+  m.q = q; m.keys = k; m.values = v; m.dout = dout;
+  m.q_sn = S[0]; m.q_sh = S[1]; m.k_sn = S[2]; m.k_sh = S[3]; m.v_sn = S[4]; m.v_sh = S[5]; m.do_sn = S[6]; m.do_sh = S[7];
+}
+
 __host__ __device__ __forceinline__ int sink_room(int sinks) { return (sinks + 7) & ~7; }
 __device__ __forceinline__ int sink_shift(int q0, int left, int room) { return max(0, q0 - left - room); }
 

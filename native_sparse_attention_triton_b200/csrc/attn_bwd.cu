@@ -834,40 +834,11 @@ static int sink_chunk(int total, int batch, int Hkv, int G, int left) {
   return chunk * per;
 }
 
-// Which rows of dK and dV are summed up in fp32: all of them, or (where a CTA of the dK/dV pass has all of a key tile's tokens) those of the
-// tiles that hold a sequence's sinks, `tiles` of them.  Row x of the grid's; false where it stands for none.
-struct SummedRows {
-  const int* cu;
-  int B, tiles, total;  // tiles < 0: all
-  __host__ __device__ long long count() const { return tiles < 0 ? total : (long long)B * tiles * 128; }
-  __device__ __forceinline__ bool row(long long x, int& n) const {
-    if (tiles < 0) {
-      n = (int)x;
-      return true;
-    }
-    const int b = (int)(x / (tiles * 128)), at = (int)(x % (tiles * 128)), start = __ldg(cu + b);
-    n = start + at;
-    return at < __ldg(cu + b + 1) - start;
-  }
-};
-
-// A warp per row of a head.
-template <int D>
-__global__ void __launch_bounds__(256) sink_zero_kernel(SummedRows r, float* dk32, float* dv32, int Hkv) {
-  const long long x = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  int n;
-  if (x >= r.count() * Hkv || !r.row(x / Hkv, n)) return;
-  const long long at = ((long long)n * Hkv + x % Hkv) * D;
-  for (int c = lane_id() * 4; c < D; c += 128) {
-    *reinterpret_cast<float4*>(dk32 + at + c) = make_float4(0.f, 0.f, 0.f, 0.f);
-    *reinterpret_cast<float4*>(dv32 + at + c) = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-}
-
 // fp32 sums of dK and dV -> storage type; a warp per row of a head.  Rows with a value that is not finite are computed one by one.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) sink_finish_kernel(DkdvParams p, SummedRows r, const __grid_constant__ SinkMaps maps, void* dk, void* dv,
                                                           long long dk_sn, long long dk_sh, long long dv_sn, long long dv_sh) {
+  wait_for_launch_before();
   long long x = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   int n;
   if (x >= r.count() * p.Hkv || !r.row(x / p.Hkv, n)) return;
@@ -912,6 +883,9 @@ static int run_sink_bwd(const void* q, const void* k, const void* v, const void*
   p.window = 1; p.stride = 1; p.causal = 1; p.left = left; p.sinks = sinks; p.rest = static_cast<const uint4*>(rest);
   p.scale2 = sm_scale * kLog2e; p.sm_scale = sm_scale;
   p.st.word = status_word();
+  const int span = (int)std::min<long long>(total, (long long)left + 128), chunk = sink_chunk(total, batch, Hkv, G, left);
+  p.summed = SummedRows{cu, batch, span > chunk ? -1 : (sinks + 127) / 128, total};
+  p.dk32 = dk32; p.dv32 = dv32;
   const int dt = DT<T>::kTmapType == CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 ? NSA_DTYPE_BF16 : NSA_DTYPE_FP16;
   const long long ds[8] = {S[0], S[1], S[2], S[3], S[4], S[5], S[8], S[9]};
   int rc = sink_dq_tc(k, v, ds, total, D, dt, p, stream);
@@ -922,27 +896,18 @@ static int run_sink_bwd(const void* q, const void* k, const void* v, const void*
   d.B = batch; d.Hq = Hq; d.Hkv = Hkv; d.G = G; d.TB = 0; d.NW = 1; d.block_size = kKeyTile;
   d.window = 1; d.stride = 1; d.causal = 1; d.left = left; d.sinks = sinks;
   d.scale2 = p.scale2; d.sm_scale = sm_scale; d.st = p.st;
-  d.chunk = sink_chunk(total, batch, Hkv, G, left);
+  d.chunk = chunk;
   d.key_slots = (int)row_tile_slots(total, batch, 7);
   d.sink_log = 13 - p.logG;  // 64 row tiles
   while (d.sink_log > 9 - p.logG && row_tile_slots(total, batch, d.sink_log) * Hkv < 148) --d.sink_log;
-  const int span = (int)std::min<long long>(total, (long long)left + 128);
-  const SummedRows summed{cu, batch, span > d.chunk ? -1 : (sinks + 127) / 128, total};
-  const long long warps = summed.count() * Hkv;
-  if (summed.tiles < 0) {
-    cudaError_t e = cudaMemsetAsync(dk32, 0, w - reinterpret_cast<uint8_t*>(dk32), stream);
-    if (e != cudaSuccess) return cuda_rc(e);
-  } else if (warps > 0) {
-    LaunchScope ls_("sink_zero", stream);
-    sink_zero_kernel<D><<<(unsigned)((warps + 7) / 8), 256, 0, stream>>>(summed, dk32, dv32, Hkv);
-  }
   rc = launch_sink_dkdv_tc<T, D>(q, dout, k, v, dk, dv, ds, S + 12, total, span, d, stream);
+  const long long warps = p.summed.count() * Hkv;
   if (rc || warps == 0) return rc;
   SinkMaps maps;
   sink_inputs(maps, q, k, v, dout, ds);
   LaunchScope ls_("sink_finish", stream);
-  sink_finish_kernel<T, D><<<(unsigned)((warps + 7) / 8), 256, 0, stream>>>(d, summed, maps, dk, dv, S[12], S[13], S[14], S[15]);
-  return cuda_rc(cudaGetLastError());
+  return cuda_rc(launch_early(sink_finish_kernel<T, D>, dim3((unsigned)((warps + 7) / 8)), 256, 0, stream, d, p.summed, maps, dk, dv, S[12], S[13],
+                              S[14], S[15]));
 }
 
 // dQ comes out of the tcgen05 dK/dV pass for these groups; the others have the mma.sync passes.

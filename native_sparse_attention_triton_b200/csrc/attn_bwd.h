@@ -26,6 +26,24 @@ __device__ __forceinline__ void red_add1(float* dst, uint32_t v) {
   asm volatile("red.global.add.f32 [%0], %1;\n" ::"l"(dst), "f"(__uint_as_float(v)) : "memory");
 }
 
+// Sliding window with sinks: which rows of dK and dV are summed up in fp32.  All of them, or (where a CTA of the dK/dV pass has all of a key
+// tile's tokens) those of the tiles that hold a sequence's sinks, `tiles` of them.
+struct SummedRows {
+  const int* cu;
+  int B, tiles, total;  // tiles < 0: all
+  __host__ __device__ long long count() const { return tiles < 0 ? total : (long long)B * tiles * 128; }
+  // row x of them; false where it stands for none
+  __device__ __forceinline__ bool row(long long x, int& n) const {
+    if (tiles < 0) {
+      n = (int)x;
+      return true;
+    }
+    const int b = (int)(x / (tiles * 128)), at = (int)(x % (tiles * 128)), start = __ldg(cu + b);
+    n = start + at;
+    return at < __ldg(cu + b + 1) - start;
+  }
+};
+
 struct DkdvParams {
   const float2* ld;    // [Nq, Hq]
   float* dk32;         // [Nk, Hkv, D] fp32 accumulators (zeroed)
@@ -71,6 +89,9 @@ struct DenseBwdParams {
   int sinks = -1;  // >= 0: sliding window with sinks (... or key < sinks)
   int rows = 0;    // of dq
   const uint4* rest = nullptr;  // what the rounding of o took away (rest_chunk in sink_keys.cuh), or nullptr
+  SummedRows summed{};          // rows of dk32 and dv32 that this pass sets to zero for the next one
+  float* dk32 = nullptr;
+  float* dv32 = nullptr;
 };
 
 struct SinkMaps;

@@ -78,6 +78,7 @@ sink_dkdv_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     return;
   }
 
+  wait_for_launch_before();
   // ---- which key tile, which tokens ----
   const int h = blockIdx.z;
   int b, qs, Lq, tile, tok_begin, tok_end, slot = blockIdx.x, st = 0;
@@ -410,8 +411,8 @@ int launch_sink_dkdv_tc(const void* q, const void* dout, const void* k, const vo
   if (e != cudaSuccess) return cuda_rc(e);
   const long long far = p.sinks > 0 ? row_tile_slots(total, p.B, p.sink_log) * ((p.sinks + 127) / 128) : 0;
   const dim3 grid((unsigned)(p.key_slots + far), (span + p.chunk - 1) / p.chunk, p.Hkv);
-  { LaunchScope ls_("sink_dkdv_tc", stream); kern<<<grid, 320, smem, stream>>>(tmQ, tmDO, tmK, tmV, p, logG, out); }
-  return cuda_rc(cudaGetLastError());
+  LaunchScope ls_("sink_dkdv_tc", stream);
+  return cuda_rc(launch_early(kern, grid, 320, smem, stream, tmQ, tmDO, tmK, tmV, p, logG, out));
 }
 
 #define NSA_INSTANTIATE(T, D)                                                                                                              \

@@ -62,9 +62,20 @@ sink_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     return;
   }
   const int QT = 128 >> p.logG, h = blockIdx.y;
-  if (warp == 0) zero_rows_behind<T, D>(p.dq, p.dq_sn, p.dq_sh, __ldg(p.cu_q + p.B), p.rows, blockIdx.x, gridDim.x, h * p.G, p.G);
+  const int batch_end = __ldg(p.cu_q + p.B);
   int b, qs, Lq, qt;
-  if (!find_row_tile(p.cu_q, p.B, 7 - p.logG, gridDim.x - 1 - blockIdx.x, b, qs, Lq, qt)) return;
+  const bool work = find_row_tile(p.cu_q, p.B, 7 - p.logG, gridDim.x - 1 - blockIdx.x, b, qs, Lq, qt);
+  if (warp == 0) zero_rows_behind<T, D>(p.dq, p.dq_sn, p.dq_sh, batch_end, p.rows, blockIdx.x, gridDim.x, h * p.G, p.G);
+  if (warp < 8) {  // a warp a row
+    for (long long x = (long long)blockIdx.x * 8 + warp; x < p.summed.count(); x += gridDim.x * 8ll) {
+      int n;
+      if (!p.summed.row(x, n)) continue;
+      const long long at = ((long long)n * p.Hkv + h) * D + lane * (D / 32);
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) p.dk32[at + c] = p.dv32[at + c] = 0.f;
+    }
+  }
+  if (!work) return;
   const int q0 = qt * QT;
   const int room = sink_room(p.sinks), shift = sink_shift(q0, p.left, room);
   const int columns = min(q0 + QT, Lq) - shift;  // of the list of keys

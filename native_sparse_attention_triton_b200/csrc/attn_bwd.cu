@@ -831,6 +831,7 @@ static int sink_chunk(int total, int batch, int Hkv, int G, int left) {
   const int span = (int)std::min<long long>(total, (long long)left + 128), all = (span + per - 1) / per;
   int chunk = all <= 160 ? all : 64;
   while (chunk > 4 && tiles * ((span + chunk * per - 1) / (chunk * per)) < 2 * 148) chunk = (chunk + 1) / 2;
+  while (span / (chunk * per) >= 65535) chunk *= 2;  // the grid's limit
   return chunk * per;
 }
 
@@ -1126,7 +1127,7 @@ extern "C" int nsa_sink_window_attn_bwd(const void* q, const void* k, const void
   if (!q || !k || !v || !o || !dout || !lse || !cu_seqlens || !dq || !dk || !dv || !workspace || !strides) return kInvalid;
   if (total_len <= 0 || batch <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || window_left < 0 || num_sinks < 0) return kInvalid;
   const int G = num_q_heads / num_kv_heads;
-  if (G > 16 || G < 1 || (G & (G - 1))) return kUnsupported;
+  if (G > 16 || G < 1 || (G & (G - 1)) || num_kv_heads > 65535) return kUnsupported;
   for (int i = 0; i < 16; ++i)
     if (strides[i] % 8) return kInvalid;
   for (const void* rows : {q, k, v, o, dout, (const void*)dq, (const void*)dk, (const void*)dv})  // read and written 16 bytes at a time

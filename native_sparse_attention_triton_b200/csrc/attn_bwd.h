@@ -27,16 +27,17 @@ __device__ __forceinline__ void red_add1(float* dst, uint32_t v) {
 }
 
 // Sliding window with sinks: which rows of dK and dV are summed up in fp32.  All of them, or (where a CTA of the dK/dV pass has all of a key
-// tile's tokens) those of the tiles that hold a sequence's sinks, `tiles` of them.
+// tile's tokens) those of the tiles that hold a sequence's sinks, `tiles` of them: counted by sequence, or through all rows where those are fewer.
 struct SummedRows {
   const int* cu;
   int B, tiles, total;  // tiles < 0: all
-  __host__ __device__ long long count() const { return tiles < 0 ? total : (long long)B * tiles * 128; }
+  __host__ __device__ bool by_sequence() const { return tiles >= 0 && (long long)B * tiles * 128 < total; }
+  __host__ __device__ long long count() const { return by_sequence() ? (long long)B * tiles * 128 : total; }
   // row x of them; false where it stands for none
   __device__ __forceinline__ bool row(long long x, int& n) const {
-    if (tiles < 0) {
+    if (!by_sequence()) {
       n = (int)x;
-      return true;
+      return tiles < 0 || (n < __ldg(cu + B) && n - __ldg(cu + find_sequence(cu, B, n)) < tiles * 128);
     }
     const int b = (int)(x / (tiles * 128)), at = (int)(x % (tiles * 128)), start = __ldg(cu + b);
     n = start + at;

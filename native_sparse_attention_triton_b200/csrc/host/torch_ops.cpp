@@ -9,6 +9,7 @@
 // Backward passes are plain autograd nodes (no Python object on the graph); they run on the engine's thread without the GIL.
 // Kernels are launched on the current stream of the tensors' device, which is made current for the duration of a call.
 #include <ATen/cuda/EmptyTensor.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -19,6 +20,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <memory>
@@ -557,6 +559,19 @@ Tensor sliding_window_attention(const Tensor& q, const Tensor& k, const Tensor& 
 }
 
 // ----------------------------------------------------------------------------------------- sliding window with sinks
+// A backward pass that is being captured cannot hand a gradient to the default stream, which is where the gradient accumulator of a leaf runs that
+// has been part of a graph built there, for as long as that graph lives.  The engine would find out behind this node's back.
+void check_captured_edges(const torch::autograd::Node& node, const at::Device& device) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  const c10::Stream outside = c10::cuda::getDefaultCUDAStream(device.index()).unwrap();
+  for (const auto& edge : node.next_edges()) {
+    const auto stream = edge.function ? edge.function->stream() : std::nullopt;
+    TORCH_CHECK(!stream || *stream != outside,
+                "an input of this captured backward pass belongs to a graph of the default stream that is still alive; "
+                "free that graph (or build it on the capturing stream) first");
+  }
+}
+
 struct SinkWindowBackward final : SavingNode {
   int left, sinks;
   double scale;
@@ -571,6 +586,7 @@ struct SinkWindowBackward final : SavingNode {
     const int64_t N = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = k.size(1);
     for (int i = 0; i < 3; ++i) out[i] = empty_like_rows(s[i]);
     if (N == 0) return out;
+    check_captured_edges(*this, q.device());
     const Tensor dout = gradient_rows(grads[0]);
     const long long bytes = nsa_sink_window_attn_bwd_workspace((int)N, (int)Hq, (int)Hkv, (int)D);
     Tensor ws = empty({bytes}, at::kByte, q.device());
@@ -600,7 +616,7 @@ Tensor sink_window_attention(const Tensor& q_in, const Tensor& k_in, const Tenso
   NSA_ASSERT(window >= 0 && sinks >= 0, "window_size and num_sinks must not be negative");
   NSA_ASSERT(q_in.size(0) < INT_MAX / 2, "at most 2^30 rows");
   const double scale = sm_scale.value_or(default_scale(q_in.size(2)));
-  NSA_ASSERT(scale > 0 && std::isfinite(scale), "sm_scale must be positive");
+  NSA_ASSERT(scale >= FLT_MIN && scale <= FLT_MAX / 2, "sm_scale must be a positive float32");
   one_device(q_in, k_in, v_in, cu);
   const bool graph = needs_graph({q_in, k_in, v_in});
   const int left = (int)std::min<int64_t>(window, INT_MAX / 2), s = (int)std::min<int64_t>(sinks, INT_MAX / 2);
@@ -1001,6 +1017,11 @@ void check_written(const Tensor& t) {
   NSA_ASSERT(!(at::GradMode::is_enabled() && t.requires_grad()), "a tensor that is written in place must not require gradients");
   at::assert_no_internal_overlap(t);
 }
+void check_written_pages(const Tensor& k, const Tensor& v) {
+  check_written(k);
+  check_written(v);
+  at::assert_no_overlap(k, v);
+}
 void wrote(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
@@ -1017,10 +1038,9 @@ Tensor paged_kv_append(const Tensor& kp, const Tensor& vp, const Tensor& table, 
   } else {
     NSA_ASSERT(k_in.size(0) == c.batch, "without cu_seqlens there is one row per sequence");
   }
+  check_written_pages(kp, vp);
   one_device(kp, vp, table, seqlens, k_in, v_in);
   if (cu) one_device(kp, *cu);
-  check_written(kp);
-  check_written(vp);
   at::NoGradGuard no_grad;
   at::AutoDispatchBelowADInplaceOrView guard;
   const Tensor k = inner_contiguous(k_in), v = inner_contiguous(v_in);
@@ -1047,16 +1067,14 @@ Tensor paged_attention_decode(const Tensor& q_in, const Tensor& kp, const Tensor
   NSA_ASSERT(!window || *window >= 0, "window_size must not be negative");
   NSA_ASSERT(sinks >= 0, "num_sinks must not be negative");
   const double scale = sm_scale.value_or(default_scale(c.d));
-  NSA_ASSERT(std::isfinite(scale), "sm_scale must be finite");
+  NSA_ASSERT(std::abs(scale) <= FLT_MAX / 2, "sm_scale must be a finite float32");
   if (weights)
     NSA_ASSERT(weights->scalar_type() == at::kFloat && weights->dim() == 3 && weights->size(0) == c.batch && weights->size(1) == c.heads &&
                    weights->size(2) >= c.capacity && weights->stride(2) == 1,
                "weights must be float32 [batch, num_kv_heads, max_pages * page_size or more] with contiguous rows");
+  if (weights) check_written(*weights);
   one_device(kp, vp, table, seqlens, q_in);
-  if (weights) {
-    one_device(kp, *weights);
-    check_written(*weights);
-  }
+  if (weights) one_device(kp, *weights);
   at::NoGradGuard no_grad;
   at::AutoDispatchBelowADInplaceOrView guard;
   const Tensor q = inner_contiguous(q_in);
@@ -1093,10 +1111,9 @@ std::tuple<Tensor, Tensor, Tensor> paged_kv_evict(const Tensor& kp, const Tensor
   NSA_ASSERT(sinks >= 0 && recent >= 0 && sinks <= budget && recent <= budget - sinks, "num_sinks and num_recent must fit into the budget");
   NSA_ASSERT(target.size(1) * c.page <= (1 << 30), "at most 2^30 rows in a sequence");
   NSA_ASSERT(target.size(1) * c.page >= std::min<int64_t>(budget, c.capacity), "new_block_table must have room for the rows that are kept");
-  one_device(kp, vp, table, seqlens, weights, target);
   NSA_ASSERT(table.data_ptr() != target.data_ptr() || c.batch == 0, "new_block_table must name other pages than block_table");
-  check_written(kp);
-  check_written(vp);
+  check_written_pages(kp, vp);
+  one_device(kp, vp, table, seqlens, weights, target);
   at::NoGradGuard no_grad;
   at::AutoDispatchBelowADInplaceOrView guard;
   Tensor after = empty({c.batch}, at::kInt, kp.device()), kept = empty({c.batch, c.heads, budget}, at::kInt, kp.device()),

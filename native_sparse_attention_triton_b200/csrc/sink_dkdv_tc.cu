@@ -23,6 +23,8 @@
 #include "sink_exact.cuh"
 #include "work_steal.cuh"
 
+#include <climits>
+
 namespace nsa {
 namespace {
 constexpr int kQStages = 3;
@@ -410,6 +412,7 @@ int launch_sink_dkdv_tc(const void* q, const void* dout, const void* k, const vo
   cudaError_t e = allow_smem(kern, smem);
   if (e != cudaSuccess) return cuda_rc(e);
   const long long far = p.sinks > 0 ? row_tile_slots(total, p.B, p.sink_log) * ((p.sinks + 127) / 128) : 0;
+  if (p.key_slots + far > INT_MAX) return kUnsupported;  // the grid's limit
   const dim3 grid((unsigned)(p.key_slots + far), (span + p.chunk - 1) / p.chunk, p.Hkv);
   LaunchScope ls_("sink_dkdv_tc", stream);
   return cuda_rc(launch_early(kern, grid, 320, smem, stream, tmQ, tmDO, tmK, tmV, p, logG, out));

@@ -98,6 +98,8 @@ def test_strides(d):
     wide[:, :c.table.shape[1]] = c.table
     c.k, c.v, c.table = both[:, 0], both[:, 1], wide[:, :c.table.shape[1]]
     _check_decode(c, 8, 50, 3, weights=True)
+    c.k = c.k[:, :, 1:2].expand(-1, -1, 4, -1)  # one head's keys for all heads
+    _check_decode(c, 8, weights=True)
     q = torch.randn(3, 16, d, device="cuda").to(BF)[:, ::2]
     value, bound, _ = paged_decode(q, c.k, c.v, c.table, c.lens)
     assert_within(ops.paged_attention_decode(q, c.k, c.v, c.table, c.seqlens), value, bound)

@@ -173,6 +173,52 @@ def test_strided_inputs_and_gradients(d, dtype):
             assert_within(got, x, t, name)
 
 
+def test_broadcast_inputs_and_gradients():
+    """Keys and values of one head (or one row) for all heads, an output gradient that is one head's: dimensions with a stride of zero."""
+    from native_sparse_attention_triton_b200 import ops
+
+    lens = [200, 133]
+    q, k, v, do = _inputs(lens, 8, 1, 128, BF, seed=9)
+    for wide_k, wide_do in ((k.expand(-1, 4, -1), do[:, :1].expand(-1, 8, -1)), (k[:1].expand(333, 4, -1), do[:1].expand(333, -1, -1))):
+        wide_v = v.expand(-1, 4, -1)
+        leaves = [x.detach().requires_grad_(True) for x in (q, wide_k, wide_v)]
+        o = ops.sink_window_attention(*leaves, _cu(lens), 40, 3)
+        grads = torch.autograd.grad([o], leaves, [wide_do])
+        value, bound = sink_window(q, wide_k, wide_v, lens, 40, 3, wide_do)
+        for name, got, x, t in zip(("o", "dq", "dk", "dv"), (o.detach(), *grads), value, bound):
+            assert_within(got, x, t, name)
+
+
+def test_all_keys_are_sinks_of_many_sequences():
+    """num_sinks far beyond the lengths: plain causal attention, all of whose key rows are summed up."""
+    _check([3, 200, 0, 1, 129, 64], 8, 2, 128, BF, 0, 10 ** 6)
+    _check([40] * 30, 4, 4, 64, FP, 3, 200)
+
+
+def test_a_captured_backward_of_leaves_that_a_living_graph_holds():
+    """Refused before the autograd engine would have the default stream wait for the one that is captured."""
+    from native_sparse_attention_triton_b200 import device_status, ops
+
+    lens, cu = [100], _cu([100])
+    q, k, v, do = _inputs(lens, 4, 2, 64, BF)
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    alive = ops.sink_window_attention(*leaves, cu, 10, 2)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(graph):
+            torch.autograd.grad([ops.sink_window_attention(*leaves, cu, 10, 2)], leaves, [do])
+    del alive
+    torch.cuda.synchronize()
+    first = [x.clone() for x in torch.autograd.grad([ops.sink_window_attention(*leaves, cu, 10, 2)], leaves, [do])]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = torch.autograd.grad([ops.sink_window_attention(*leaves, cu, 10, 2)], leaves, [do])
+    graph.replay()
+    for a, b in zip(first, grads):
+        assert torch.allclose(a.float(), b.float(), rtol=2 ** -6, atol=1e-5)
+    assert device_status() == 0
+
+
 def test_no_tokens():
     from native_sparse_attention_triton_b200 import ops
 

@@ -24,7 +24,7 @@ def test_sink_window_gets_as_far_as_the_device():
     dict(q=torch.zeros(10, 4, 128)), dict(k=torch.zeros(10, 2, 128).half()), dict(q=torch.zeros(10, 4 * 128).bfloat16()),
     dict(q=torch.zeros(9, 4, 128).bfloat16()), dict(v=torch.zeros(10, 1, 128).bfloat16()), dict(q=torch.zeros(10, 3, 128).bfloat16()),
     dict(q=torch.zeros(10, 4, 64).bfloat16()), dict(cu=torch.tensor([0, 10])), dict(cu=torch.tensor([0], dtype=I)), dict(window=-1), dict(sinks=-1),
-    dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(cu=torch.tensor([[0, 10]], dtype=I)),
+    dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=1e-60), dict(scale=1e60), dict(cu=torch.tensor([[0, 10]], dtype=I)),
     {x: torch.zeros(10, 2, 96).bfloat16() for x in "qkv"}, dict(k=torch.zeros(10, 0, 128).bfloat16(), v=torch.zeros(10, 0, 128).bfloat16())])
 def test_sink_window_refuses(change):
     with pytest.raises(AssertionError):
@@ -85,7 +85,7 @@ def test_rows_that_append_refuses(change):
 
 @pytest.mark.parametrize("change", [
     dict(q=torch.zeros(2, 8, 128).bfloat16()), dict(q=torch.zeros(3, 7, 128).bfloat16()), dict(q=torch.zeros(3, 8, 128).half()),
-    dict(q=torch.zeros(3, 8, 64).bfloat16()), dict(window=-1), dict(sinks=-1), dict(scale=float("inf")),
+    dict(q=torch.zeros(3, 8, 64).bfloat16()), dict(window=-1), dict(sinks=-1), dict(scale=float("inf")), dict(scale=1e60),
     dict(weights=torch.zeros(3, 2, 31)), dict(weights=torch.zeros(3, 4, 32)), dict(weights=torch.zeros(3, 2, 32).half())])
 def test_queries_that_decode_refuses(change):
     with pytest.raises(AssertionError):
@@ -106,6 +106,23 @@ def test_evictions_that_are_refused(change):
         CALLS["evict"](_cache(**change))
 
 
+@pytest.mark.parametrize("call", ["append", "evict"])
+def test_caches_that_cannot_be_written(call):
+    pages = torch.zeros(6, 16, 2, 128).bfloat16()
+    for kp, vp in ((pages, pages), (pages.narrow(0, 0, 1).expand(6, 16, 2, 128), pages), (pages[:, :, :1].expand(6, 16, 2, 128), pages)):
+        with pytest.raises(RuntimeError, match="unsupported operation"):
+            CALLS[call](_cache(kp=kp, vp=vp))
+    with pytest.raises(AssertionError):
+        CALLS[call](_cache(kp=pages.clone().requires_grad_(True)))
+
+
+def test_weights_that_cannot_be_added_to():
+    with pytest.raises(RuntimeError, match="unsupported operation"):
+        CALLS["decode"](_cache(weights=torch.zeros(3, 1, 32).expand(3, 2, 32)))
+    with pytest.raises(AssertionError):
+        CALLS["decode"](_cache(weights=torch.zeros(3, 2, 32, requires_grad=True)))
+
+
 def test_c_interface_refuses_before_it_touches_a_device():
     lib = _lib.lib()
     z = _lib.strides_array(*[8] * 16)
@@ -119,6 +136,7 @@ def test_c_interface_refuses_before_it_touches_a_device():
     assert lib.nsa_paged_attn_decode(*[p] * 6, None, p, 1 << 40, 1, 17, 1, 128, 1, 1, 1, 0, 0, z, 1.0, 0, None) == -2
     assert lib.nsa_paged_kv_append(*[p] * 8, 1, 1, 1, 96, 1, 1, 1, z, None) == -2
     assert lib.nsa_paged_kv_evict(*[p] * 9, 1, 1, 128, 1, 1, 1, 1, 1, 4, 5, 0, z, None) == -1                       # sinks beyond the budget
+    assert lib.nsa_sink_window_attn_fwd(*[p] * 7, 1, 1, 65536, 65536, 128, 1, 1, z, 1.0, 0, None) == -2                 # the grid's second dimension
     odd = _lib.strides_array(*[4] * 16)
     assert lib.nsa_sink_window_attn_fwd(*[p] * 7, 1, 1, 1, 1, 128, 1, 1, odd, 1.0, 0, None) == -1
     assert lib.nsa_sink_window_attn_bwd(*[p] * 12, 0, 1, 1, 1, 1, 128, 1, 1, z, 1.0, 0, None) == -3

@@ -544,11 +544,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     const PairSpan w = open[warp];
     if (w.pair >= 0) {
       const int first = shares.owner(w.start), n = shares.owner(w.stop - 1) - first + 1;
-      if (lane == 0) {  // (one thread's fences: the CTA's barriers stand on either side)
-        __threadfence();
-        last_of[warp] = atomicInc(p.ctrl + first, (unsigned)(n - 1)) == (unsigned)(n - 1) ? n : 0;
+      if (lane == 0) {  // (released and acquired by one thread: the CTA's barriers stand on either side)
+        unsigned came;
+        asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;\n" : "=r"(came) : "l"(p.ctrl + first), "r"((unsigned)(n - 1)) : "memory");
+        last_of[warp] = came == (unsigned)(n - 1) ? n : 0;
         first_of[warp] = first;
-        __threadfence();
       }
     } else if (lane == 0) {
       last_of[warp] = 0;

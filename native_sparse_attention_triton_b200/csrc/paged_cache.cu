@@ -37,6 +37,7 @@ template <int D>
 __global__ void __launch_bounds__(256) paged_append_kernel(PagedAppendParams p) {
   constexpr int CH = D / 8;
   const int lane = lane_id();
+  wait_for_launch_before();
   for (int b = blockIdx.x * 256 + threadIdx.x; b < p.B; b += gridDim.x * 256)
     p.after[b] = min(p.cap, __ldg(p.held + b) + (p.cu ? __ldg(p.cu + b + 1) - __ldg(p.cu + b) : 1));
   const int n = blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -132,6 +133,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(PagedEvict
   __shared__ uint32_t sums[4][kSelectThreads / 32];
   __shared__ uint32_t s_digit, s_rank;
   const int b = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv, tid = threadIdx.x;
+  wait_for_launch_before();
   const int len = __ldg(p.seqlens + b), L = max(0, min(len, p.cap)), m = min(L, p.budget);
   if (len > p.cap && tid == 0) p.st.raise(kErrBadIndex);
   const float* w = p.w + b * p.w_sb + h * p.w_sh;
@@ -315,9 +317,7 @@ extern "C" int nsa_paged_kv_append(void* k_pages, void* v_pages, const int* bloc
   const int grid = std::max(1, (total_len + 7) / 8);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   LaunchScope ls_("paged_append", s);
-  if (head_dim == 128) paged_append_kernel<128><<<grid, 256, 0, s>>>(p);
-  else paged_append_kernel<64><<<grid, 256, 0, s>>>(p);
-  return cuda_rc(cudaGetLastError());
+  return cuda_rc(launch_early(head_dim == 128 ? paged_append_kernel<128> : paged_append_kernel<64>, dim3(grid), 256, 0, s, p));
 }
 
 extern "C" int nsa_paged_kv_evict(void* k_pages, void* v_pages, const int* block_table, const int* seqlens, const float* weights,
@@ -349,8 +349,11 @@ extern "C" int nsa_paged_kv_evict(void* k_pages, void* v_pages, const int* block
   p.budget = budget; p.sinks = num_sinks; p.recent = num_recent;
   p.st.word = status_word();
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  { LaunchScope ls_("evict_select", s); evict_select_kernel<<<batch * num_kv_heads, kSelectThreads, 0, s>>>(p); }
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e;
+  {
+    LaunchScope ls_("evict_select", s);
+    e = launch_early(evict_select_kernel, dim3(batch * num_kv_heads), kSelectThreads, 0, s, p);
+  }
   if (e != cudaSuccess) return cuda_rc(e);
   const dim3 grid(batch * num_kv_heads, (unsigned)((most + 127) / 128));
   LaunchScope ls_("evict_move", s);

@@ -204,6 +204,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   uint64_t* full = full_bars + warp * kPagedStages;
   unsigned* seen_sm = seen + warp * kPagedStages;
 
+  wait_for_launch_before();
   // ---- this CTA's and this warp's run of tiles ----
   const unsigned total = count_tiles<THREADS>(p, before, warp_sums);
   const int nc = (int)min(gridDim.x, (total + WARPS - 1) / WARPS);  // CTAs with work
@@ -660,8 +661,10 @@ static int launch_paged_decode(PagedDecodeParams p, float* weights, long long w_
   if (e != cudaSuccess) return cuda_rc(e);
   const long long most = (long long)p.B * p.Hkv * ((p.cap + kPagedRows - 1) / kPagedRows);
   const int grid = (int)std::min<long long>(num_sms(), (most + WARPS - 1) / WARPS);
-  { LaunchScope ls_("paged_decode", stream); kern<<<grid, WARPS * 32, smem, stream>>>(tmK, tmV, p); }
-  e = cudaGetLastError();
+  {
+    LaunchScope ls_("paged_decode", stream);
+    e = launch_early(kern, grid, WARPS * 32, smem, stream, tmK, tmV, p);
+  }
   if (e != cudaSuccess || !weights) return cuda_rc(e);
   LaunchScope ls_("paged_weights", stream);
   return cuda_rc(launch_early(paged_weights_kernel, dim3(p.B * p.Hkv, (p.cap + 256 * kWeightRows - 1) / (256 * kWeightRows)), 256, 0, stream, p, weights, w_sb, w_sh));

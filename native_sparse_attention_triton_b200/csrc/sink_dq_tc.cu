@@ -62,6 +62,7 @@ sink_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     return;
   }
   const int QT = 128 >> p.logG, h = blockIdx.y;
+  wait_for_launch_before();
   const int batch_end = __ldg(p.cu_q + p.B);
   int b, qs, Lq, qt;
   const bool work = find_row_tile(p.cu_q, p.B, 7 - p.logG, gridDim.x - 1 - blockIdx.x, b, qs, Lq, qt);
@@ -378,8 +379,8 @@ static int launch_sink_dq(const void* k, const void* v, const long long* S, int 
   cudaError_t e = allow_smem(kern, smem, /*shared_sm=*/true);
   if (e != cudaSuccess) return cuda_rc(e);
   const dim3 grid((unsigned)row_tile_slots(total, p.B, 7 - p.logG), p.Hkv);
-  { LaunchScope ls_("sink_dq_tc", stream); kern<<<grid, 320, smem, stream>>>(tmQ, tmDO, tmK, tmV, tmDQ, p, split); }
-  return cuda_rc(cudaGetLastError());
+  LaunchScope ls_("sink_dq_tc", stream);
+  return cuda_rc(launch_early(kern, grid, 320, smem, stream, tmQ, tmDO, tmK, tmV, tmDQ, p, split));
 }
 
 int sink_dq_tc(const void* k, const void* v, const long long* strides, int total, int head_dim, int dtype, DenseBwdParams p, cudaStream_t stream) {

@@ -78,6 +78,7 @@ sink_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     return;
   }
   const int QT = 128 >> p.logG, h = blockIdx.y;
+  wait_for_launch_before();
   const int batch_end = __ldg(p.cu + p.B);
   int b, qs, Lq, qt;
   const bool work = find_row_tile(p.cu, p.B, 7 - p.logG, gridDim.x - 1 - blockIdx.x, b, qs, Lq, qt);  // long rows first
@@ -371,8 +372,8 @@ static int launch_sink_fwd(const void* q, const void* k, const void* v, const lo
   cudaError_t e = allow_smem(kern, smem, /*shared_sm=*/true);
   if (e != cudaSuccess) return cuda_rc(e);
   const dim3 grid((unsigned)row_tile_slots(p.rows, p.B, 7 - p.logG), p.Hkv);
-  { LaunchScope ls_("sink_fwd_tc", stream); kern<<<grid, kThreads, smem, stream>>>(tmQ, tmK, tmV, tmO, p, split); }
-  return cuda_rc(cudaGetLastError());
+  LaunchScope ls_("sink_fwd_tc", stream);
+  return cuda_rc(launch_early(kern, grid, kThreads, smem, stream, tmQ, tmK, tmV, tmO, p, split));
 }
 
 }  // namespace nsa

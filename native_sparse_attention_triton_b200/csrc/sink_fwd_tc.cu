@@ -12,7 +12,7 @@
 // A row tile sees few keys (9 tiles of 64 at a window of 512), so what bounds the pass is a CTA's beginning and end and the chain of a tile's softmax.
 // Hence 96 KB of shared memory and 256 columns of tensor memory, so that two CTAs share an SM and one works while the other loads, waits or
 // stores; and two logit buffers, so that the products of a tile run under the softmax of the one before it.  64q/4kv, window 512, 4 sinks, 32 768
-// tokens, with o's rest for the backward pass: 895 us; of a CTA's 22 600 clocks 4000 pass until its first logits, 900 and a hand-over of 300 a tile of
+// tokens, with o's rest and one part of P (below): 895 us; of a CTA's 22 600 clocks 4000 pass until its first logits, 900 and a hand-over of 300 a tile of
 // 64 (2200 the first, 1700 the last, which are masked), 4900 from the last P to the end.  Two threads per row made a tile's softmax no shorter
 // (920 us: the exponential unit then serves four warps); the dense forward's organisation (two row tiles in one CTA, tiles of 128 keys, one logit
 // buffer each, persistent) took 911 us without the rest and 1074 with it.
@@ -49,7 +49,11 @@ struct SinkFwdParams {
   Status st;
 };
 
-template <typename T, int D>
+// REST: for a backward pass.  The probabilities are then two 16-bit parts, p = hi + lo, and P V two products: the backward pass needs sum_d o dO
+// next to single dO v, and one part's rounding in o (2^-9 of each p in bf16) would add to dS, which is rounded itself, more than half as much
+// again.  Packed 32 K tokens: 915 -> 1085 us; errors against 64 bits, in
+// units of the final rounding: o 1.36 -> 1.00, dQ 1.50 -> 1.43, dK 1.46 -> 1.41 (1.41 is what rounding dS alone leaves).
+template <typename T, int D, bool REST>
 __global__ void __launch_bounds__(kThreads, 2)
 sink_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const __grid_constant__ CUtensorMap tmO, SinkFwdParams p, const __grid_constant__ SinkMaps split) {
@@ -168,6 +172,11 @@ sink_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; ++kk)
           umma_ts(tmem + kO, tmem + (i & 1) * kKeys + kk * 8, umma_desc_mnmajor(v_base + s * KEY_BYTES + kk * 2048, KEY_PANEL), idesc_o, i > 0 || kk > 0);
+        if (REST) {
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            umma_ts(tmem + kO, tmem + (i & 1) * kKeys + 32 + kk * 8, umma_desc_mnmajor(v_base + s * KEY_BYTES + kk * 2048, KEY_PANEL), idesc_o, true);
+        }
         umma_commit(v_empty + s);
         umma_commit(pv_done);
       }
@@ -184,8 +193,8 @@ sink_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16);
     // columns that all rows of the tile see, if all of them are rows
     const int inner0 = q0 + QT - 1 - p.left - shift, inner1 = q0 + QT <= Lq ? q0 + 1 - shift : -1;
-    // The output is divided by the sum of the ROUNDED probabilities of tiles that a row does not see in full: where it sees few keys, one of
-    // nearly all the weight then leaves no rounding in o, which the backward pass's sum o dO needs (rest_chunk).  Log-sum-exp has the exact sum.
+    // With one part the output is divided by the sum of the ROUNDED probabilities of tiles that a row does not see in full: where it sees few keys,
+    // one of nearly all the weight then leaves no rounding in o.  Log-sum-exp has the exact sum.
     float m_ref = -INFINITY, l = 0.f, l_rounded = 0.f;
     for (int i = 0; i < ntiles; ++i) {
       const uint32_t s_base = lane_base + (i & 1) * kKeys;
@@ -240,7 +249,7 @@ sink_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       }
       const float nm = m_ref == -INFINITY ? 0.f : -m_ref;
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      uint32_t pk[32];
+      uint32_t pk[32], lo[32];
       auto exps = [&](auto full_tag) {
         constexpr bool FULL = decltype(full_tag)::value;
 #pragma unroll
@@ -250,14 +259,19 @@ sink_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           const float2 e = FULL && j % kPolyEvery == kPolyEvery - 1 ? exp2_poly2(x) : make_float2(fast_exp2(x.x), fast_exp2(x.y));
           sum[j & 1] = fadd2(sum[j & 1], e);
           pk[j] = DT<T>::pack(e.x, e.y);
+          if (REST) {
+            const float2 r = DT<T>::unpack(pk[j]);
+            lo[j] = DT<T>::pack(e.x - r.x, e.y - r.y);
+          }
         }
       };
       if (all) exps(std::true_type{});
       else exps(std::false_type{});
       tmem_st32(s_base, pk);
+      if (REST) tmem_st32(s_base + 32, lo);
       const float more = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       l += more;
-      if (all) {
+      if (REST || all) {
         l_rounded += more;
       } else {
         float2 r[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -300,7 +314,7 @@ sink_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           const float2 h2 = DT<T>::unpack(hi[e]);
           lo[e] = DT<T>::pack(x.x - h2.x, x.y - h2.y);
         }
-        if (p.rest && valid) rest[q8 * rest_step] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (REST && valid) rest[q8 * rest_step] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         if (staged)
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(smem_u32(q_sm) + c * ROW_PANEL + row * 128 + ((q8 ^ (row & 7)) << 4)),
                        "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
@@ -317,7 +331,7 @@ sink_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       const float4 x = exact_query_row<T, D, false>(&split, qs, t, hd, h, p.left, p.sinks, p.scale2, 0.f, __shfl_sync(0xffffffffu, lse, src), 0.f);
       if (staged) store_lane_elements_swizzled<T, D, ROW_PANEL>(q_sm, rw, x);
       else store_lane_elements<T, D>(static_cast<T*>(p.o) + (long long)(qs + t) * p.o_sn + (long long)hd * p.o_sh, x);
-      if (p.rest) {
+      if (REST) {
         const int at = lane * (D / 32);  // element; a chunk has eight
         T* chunk = reinterpret_cast<T*>(p.rest + rest_chunk(at / 8, h, p.Hkv, p.rows, qs + t, p.G, hd - h * p.G));
         const float2 a = DT<T>::unpack(DT<T>::pack(x.x, x.y)), c = DT<T>::unpack(DT<T>::pack(x.z, x.w));
@@ -368,7 +382,7 @@ static int launch_sink_fwd(const void* q, const void* k, const void* v, const lo
   if (!rc) rc = make_sink_maps(split, DT<T>::kTmapType, q, k, v, nullptr, S, D, p.Hkv, p.rows, p.sinks, kKeys);
   if (rc) return rc;
   const size_t smem = (size_t)(128 + 2 * kStages * kKeys) * D * 2 + 18 * sizeof(uint64_t);
-  auto kern = sink_fwd_tc_kernel<T, D>;
+  auto kern = p.rest ? sink_fwd_tc_kernel<T, D, true> : sink_fwd_tc_kernel<T, D, false>;
   cudaError_t e = allow_smem(kern, smem, /*shared_sm=*/true);
   if (e != cudaSuccess) return cuda_rc(e);
   const dim3 grid((unsigned)row_tile_slots(p.rows, p.B, 7 - p.logG), p.Hkv);

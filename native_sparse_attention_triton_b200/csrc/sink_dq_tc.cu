@@ -8,7 +8,8 @@
 //
 // A row tile sees few key tiles (9 of 64 at a window of 512), so what bounds the pass is not its products but a CTA's beginning and end and
 // the chain S -> P -> dP -> dS -> dQ of each tile.  Hence tiles of 64 keys instead of the dense pass's 128: with 112 KB of shared memory and
-// 256 columns of tensor memory two CTAs share an SM and each works while the other waits, and less of the last tile is empty.
+// 256 columns of tensor memory two CTAs share an SM and each works while the other waits, and less of the last tile is empty.  64q/4kv, window 512, 4 sinks, 32 768 tokens: 1390 us against 1650 with
+// tiles of 128 and one CTA; of a CTA's 36 000 clocks 9000 pass before its first dS (dO, o and its rest come from memory), 2500 a tile of 64.
 //   warps 0..7 : two threads per row (32 key columns each)
 //   warp 8     : TMA producer (Q, dO; K ring of two, V ring of one);   warp 9 : TMEM allocation and MMA issue (one thread)
 #include "attn_bwd.h"

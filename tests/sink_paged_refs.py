@@ -56,7 +56,8 @@ def sink_window(q, k, v, lens, window, sinks, do=None, scale=None):
             g_ = do[part, head].double()
             dp, delta = g_ @ vh.T, (o * g_).sum(1, keepdim=True)
             ds = p * (dp - delta) * scale
-            # of dS: its rounding, that of o in delta (o is kept as two 16-bit numbers, but the roundings of P in it stay), and the
+            # of dS: its rounding, that of o in delta (o is kept as two 16-bit numbers; one rounding of each P in it is allowed for, which the
+            # two parts of P that a forward has for a backward pass stay far below), and the
             # 32-bit arithmetic of its parts
             o_kept = o_err - (h - h * h) * o.abs()
             err = h * ds.abs() + u * see + p * scale * (o_kept * g_.abs()).sum(1, keepdim=True) + SLACK * p * scale * (g_.abs() @ vh.abs().T + delta.abs())

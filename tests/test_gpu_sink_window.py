@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.sink_paged_refs import assert_within, sink_window, window_mask
+from tests.sink_paged_refs import SLACK, assert_within, half_step, least_step, sink_window, window_mask
 
 pytestmark = pytest.mark.gpu
 
@@ -278,3 +278,24 @@ def test_on_a_stream_of_its_own_and_captured():
     value, bound = sink_window(*other[:3], lens, 64, 4, other[3])
     for got, x, t in zip(outs, value, bound):
         assert_within(got, x, t)
+
+
+@pytest.mark.parametrize("d,dtype", [(128, BF), (64, BF), (128, FP), (64, FP)])
+@pytest.mark.parametrize("lens,window,sinks", [([9, 1, 2], 3, 1), ([700, 130], 100, 4), ([513], 512, 64)])
+def test_an_output_for_a_backward_pass_has_the_probabilities_in_two_parts(d, dtype, lens, window, sinks):
+    """Each p = hi + lo is off by at most h * h (lo, at most h of p, is rounded itself), or by the least step of the type; what is left is the
+    output's own rounding, h of it, and SLACK.  One part would be off by h of each p."""
+    from native_sparse_attention_triton_b200 import ops
+
+    q, k, v, _ = _inputs(lens, 8, 2, d, dtype, seed=3)
+    o = ops.sink_window_attention(q.requires_grad_(True), k, v, _cu(lens), window, sinks).detach()
+    q, h, u, start = q.detach(), half_step(dtype), least_step(dtype), 0
+    for n in lens:
+        part = slice(start, start + n)
+        see = window_mask(n, window, sinks, "cuda")
+        for head in range(8):
+            vh = v[part, head // 4].double()
+            p = torch.softmax((q[part, head].double() @ k[part, head // 4].double().T * d ** -0.5).masked_fill(~see, -float("inf")), 1)
+            x = p @ vh
+            assert_within(o[part, head], x, h * x.abs() + u + (h * h + SLACK) * (p @ vh.abs()) + u * (see.double() @ vh.abs()), "o")
+        start += n

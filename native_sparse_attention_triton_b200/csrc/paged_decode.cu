@@ -23,8 +23,10 @@
 #include "dispatch.h"
 #include "host_util.h"
 #include "nsa_b200.h"
+#include "sink_exact.cuh"
 
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 namespace nsa {
@@ -185,10 +187,43 @@ struct PairSpan {
   unsigned start, stop;
 };
 
+// Output of query head h * G + g of sequence b by 32-bit probabilities over the rows it sees, from its maximum m and sum l; a warp.  A row whose
+// tiles gave it a value that is not finite is computed again here: hi * inf + lo * inf is no number where lo is zero or below, nor is the product
+// of infinity and a probability that 16 or 32 bits round to zero (none is zero: at least FLT_MIN, which no finite value shows).  Some 100 clocks a
+// row of the cache, which only those that hold such values pay.
+template <typename T, int D>
+__device__ __noinline__ void exact_decode_row(const PagedDecodeParams* p, int b, int h, int g, float m, float l) {
+  const Rows rows = visible_rows(*p, b);
+  const int head = h * p->G + g, lane = lane_id();
+  float q[4], k[4], v[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
+  lane_elements<T, D>(q, p->q, (long long)b * p->q_sb + (long long)head * p->q_sh);
+  for (int t = 0; t < rows.n; ++t) {
+    const int j = (t < rows.gap_at ? t : t + rows.gap) * kPagedRows + lane;
+    const bool in = j < rows.len && (j >= rows.first || j < rows.head);
+    const int page = in ? __ldg(p->table + (long long)b * p->t_sb + j / p->page) : -1;
+    for (unsigned see = __ballot_sync(0xffffffffu, (unsigned)page < (unsigned)p->num_pages); see; see &= see - 1) {
+      const int src = __ffs(see) - 1;
+      const long long pg = __shfl_sync(0xffffffffu, page, src), slot = __shfl_sync(0xffffffffu, j % p->page, src);
+      lane_elements<T, D>(k, p->k, pg * p->k_sp + slot * p->k_ss + (long long)h * p->k_sh);
+      lane_elements<T, D>(v, p->v, pg * p->v_sp + slot * p->v_ss + (long long)h * p->v_sh);
+      const float x = warp_dot(q, k) * p->scale2;
+      float w = fast_exp2(x - m);
+      if (w == 0.f && x > -INFINITY) w = FLT_MIN;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, v[e], acc[e]);
+    }
+  }
+  const float inv = 1.f / l;
+  __syncwarp();  // what the tiles gave has been written
+  store_lane_elements<T, D>(static_cast<T*>(p->o) + (long long)b * p->o_sb + (long long)head * p->o_sh,
+                            make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv));
+}
+
 // TMA: tiles come as boxes of p.box rows; else row by row with cp.async (pages whose size has no factor of 8).
 template <typename T, int D, bool TMA>
 __global__ void __launch_bounds__(PagedShape<D>::kThreads, 1)
-paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, PagedDecodeParams p) {
+paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                    const __grid_constant__ PagedDecodeParams p) {
   constexpr int ROWS = kPagedRows, NT = ROWS / 8, CH = D / 8;  // 16-byte chunks of a row
   constexpr int WARPS = PagedShape<D>::kWarps, THREADS = WARPS * 32, TILE = PagedShape<D>::kTileBytes, RING = PagedShape<D>::kRing;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -431,12 +466,20 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int g = r0 + half * 8;
+            float zero = 0.f;  // 0 times each value
             if (g < p.G) {
               T* row = ob + (long long)g * p.o_sh + c0;
 #pragma unroll
-              for (int j = 0; j < D / 8; ++j)
+              for (int j = 0; j < D / 8; ++j) {
+                zero = fmaf(o[j][2 * half + 1], 0.f, fmaf(o[j][2 * half], 0.f, zero));
                 *reinterpret_cast<uint32_t*>(row + j * 8) = DT<T>::pack(o[j][2 * half] * inv[half], o[j][2 * half + 1] * inv[half]);
+              }
               if (p.lse && (lane & 3) == 0) p.lse[(long long)pair * p.G + g] = l[half] > 0.f ? m[half] + log2f(l[half]) : -INFINITY;
+            }
+            for (unsigned redo = __ballot_sync(0xffffffffu, l[half] > 0.f && zero != 0.f); redo;) {
+              const int src = (__ffs(redo) - 1) & ~3;  // a row is four lanes'
+              redo &= ~(15u << src);
+              exact_decode_row<T, D>(&p, cur.b, cur.h, (src >> 2) + half * 8, __shfl_sync(0xffffffffu, m[half], src), __shfl_sync(0xffffffffu, l[half], src));
             }
           }
         } else {
@@ -481,6 +524,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 #pragma unroll
     for (int c = 0; c < EPL; c += 2) row[c / 2] = DT<T>::pack(val[c] * inv, val[c + 1] * inv);
     if (p.lse && lane == 0) p.lse[(long long)pair * p.G + g] = ll > 0.f ? mm + log2f(ll) : -INFINITY;
+    float zero = 0.f;  // 0 times each value
+#pragma unroll
+    for (int c = 0; c < EPL; ++c) zero = fmaf(val[c], 0.f, zero);
+    if (__any_sync(0xffffffffu, ll > 0.f && zero != 0.f)) exact_decode_row<T, D>(&p, b, h, g, mm, ll);
   };
   {
     auto part_at = [&](int i) { return (i & 1) ? reinterpret_cast<const Part<D>*>(smem + (i >> 1) * RING) : head_parts + (i >> 1); };

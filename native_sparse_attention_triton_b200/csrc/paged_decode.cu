@@ -219,6 +219,9 @@ __device__ __noinline__ void exact_decode_row(const PagedDecodeParams* p, int b,
                             make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv));
 }
 
+// Log-sum-exp of a row: of nothing it is minus infinity, and where the sum is no number the log is none, so that what is made of it says so too.
+__device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? -INFINITY : m + log2f(l); }
+
 // TMA: tiles come as boxes of p.box rows; else row by row with cp.async (pages whose size has no factor of 8).
 template <typename T, int D, bool TMA>
 __global__ void __launch_bounds__(PagedShape<D>::kThreads, 1)
@@ -474,7 +477,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 zero = fmaf(o[j][2 * half + 1], 0.f, fmaf(o[j][2 * half], 0.f, zero));
                 *reinterpret_cast<uint32_t*>(row + j * 8) = DT<T>::pack(o[j][2 * half] * inv[half], o[j][2 * half + 1] * inv[half]);
               }
-              if (p.lse && (lane & 3) == 0) p.lse[(long long)pair * p.G + g] = l[half] > 0.f ? m[half] + log2f(l[half]) : -INFINITY;
+              if (p.lse && (lane & 3) == 0) p.lse[(long long)pair * p.G + g] = log_sum(m[half], l[half]);
             }
             for (unsigned redo = __ballot_sync(0xffffffffu, l[half] > 0.f && zero != 0.f); redo;) {
               const int src = (__ffs(redo) - 1) & ~3;  // a row is four lanes'
@@ -523,7 +526,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     uint32_t* row = reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + (long long)b * p.o_sb + (long long)(h * p.G + g) * p.o_sh + lane * EPL);
 #pragma unroll
     for (int c = 0; c < EPL; c += 2) row[c / 2] = DT<T>::pack(val[c] * inv, val[c + 1] * inv);
-    if (p.lse && lane == 0) p.lse[(long long)pair * p.G + g] = ll > 0.f ? mm + log2f(ll) : -INFINITY;
+    if (p.lse && lane == 0) p.lse[(long long)pair * p.G + g] = log_sum(mm, ll);
     float zero = 0.f;  // 0 times each value
 #pragma unroll
     for (int c = 0; c < EPL; ++c) zero = fmaf(val[c], 0.f, zero);

@@ -36,7 +36,8 @@ def paged_attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     seqlens[b] - 1 - j <= window_size, or j < num_sinks: what the query sees in sink_window_attention.  A sequence without rows gets zeros.
     weights float32 [batch, num_kv_heads, max_pages * page_size or more]: the probabilities that each visible row receives, summed over
     the query heads of its key/value head, are added in place (paged_kv_evict goes by them); other entries are left as they are.
-    Not differentiable.
+    Values that are not finite reach what the definition makes depend on them: a head whose logits hold NaN has no output, and adds NaN to the
+    weights of the rows it sees.  Not differentiable.
     """
     return _lib.host().paged_attention_decode(q, k_pages, v_pages, block_table, seqlens, sm_scale,
                                               None if window_size is None else int(window_size), int(num_sinks), weights)

@@ -95,3 +95,23 @@ def test_with_a_window_and_sinks():
     _row(c, c.v, 0, 2000)[:] = NAN           # in neither
     value = _check(c, 8, 100, 4, weights=True)
     assert value[:, :, 2].isposinf().all() and value[:, :, 7].isnan().all() and value[0, 0, 3].isfinite()
+
+
+@pytest.mark.parametrize("d,dtype", [(128, BF), (64, FP)])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_a_visible_key_that_is_no_number(shape, d, dtype):
+    """Neither the heads that see it nor the sums that they add to have a number."""
+    c = Cache(SHAPES[shape], 2, d, 16, dtype)
+    for b in range(0, len(c.lens), 2):
+        _row(c, c.k, b, (b * 11) % c.lens[b])[1, 6] = NAN
+    value = _check(c, 8, weights=True)
+    assert value[0, 4:].isnan().all() and value[0, :4].isfinite().all()
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_a_query(shape):
+    c = Cache(SHAPES[shape], 2, 128, 16, BF)
+    q = c.queries(8)
+    q[0, 3, 5], q[-1, 6, 0] = NAN, NAN
+    value = _check(c, 8, weights=True, q=q)
+    assert value[0, 3].isnan().all() and value[0, 2].isfinite().all()

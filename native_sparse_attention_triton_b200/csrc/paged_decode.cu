@@ -219,8 +219,11 @@ __device__ __noinline__ void exact_decode_row(const PagedDecodeParams* p, int b,
                             make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv));
 }
 
-// Log-sum-exp of a row: of nothing it is minus infinity, and where the sum is no number the log is none, so that what is made of it says so too.
-__device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? -INFINITY : m + log2f(l); }
+// 1 / sum and log-sum-exp of a row.  A sum of zero is one over nothing (its maximum is -infinity; outputs are zero), or over logits that are all
+// -infinity (its maximum is kNothingYet): no number then, as where the sum itself is none.
+constexpr float kNothingYet = -FLT_MAX;
+__device__ __forceinline__ float inverse_sum(float m, float l) { return l != 0.f ? 1.f / l : m == -INFINITY ? 0.f : NAN; }
+__device__ __forceinline__ float log_sum(float m, float l) { return l != 0.f ? m + log2f(l) : m == -INFINITY ? -INFINITY : NAN; }
 
 // TMA: tiles come as boxes of p.box rows; else row by row with cp.async (pages whose size has no factor of 8).
 template <typename T, int D, bool TMA>
@@ -406,7 +409,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       float base[2], corr[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float top = fmaxf(m[r], quad_max(mx[r]));
+        const float top = fmaxf(fmaxf(m[r], see ? kNothingYet : -INFINITY), quad_max(mx[r]));
         base[r] = top == -INFINITY ? 0.f : top;
         corr[r] = fast_exp2(m[r] - base[r]);
         m[r] = top;
@@ -465,7 +468,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         const int r0 = lane >> 2;
         if (pair_ends && seg_t0 == 0) {
           T* ob = static_cast<T*>(p.o) + (long long)cur.b * p.o_sb + (long long)cur.h * p.G * p.o_sh;
-          const float inv[2] = {l[0] > 0.f ? 1.f / l[0] : 0.f, l[1] > 0.f ? 1.f / l[1] : 0.f};
+          const float inv[2] = {inverse_sum(m[0], l[0]), inverse_sum(m[1], l[1])};
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int g = r0 + half * 8;
@@ -522,7 +525,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   };
   auto write_row = [&](int pair, int g, const float (&val)[EPL], float mm, float ll) {
     const int b = pair / p.Hkv, h = pair - b * p.Hkv;
-    const float inv = ll > 0.f ? 1.f / ll : 0.f;
+    const float inv = inverse_sum(mm, ll);
     uint32_t* row = reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + (long long)b * p.o_sb + (long long)(h * p.G + g) * p.o_sh + lane * EPL);
 #pragma unroll
     for (int c = 0; c < EPL; c += 2) row[c / 2] = DT<T>::pack(val[c] * inv, val[c + 1] * inv);

@@ -115,3 +115,25 @@ def test_a_query(shape):
     q[0, 3, 5], q[-1, 6, 0] = NAN, NAN
     value = _check(c, 8, weights=True, q=q)
     assert value[0, 3].isnan().all() and value[0, 2].isfinite().all()
+
+
+@pytest.mark.parametrize("d,dtype", [(128, BF), (64, FP)])
+@pytest.mark.parametrize("bad", [INF, -INF, NAN])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_a_visible_key(shape, bad, d, dtype):
+    """Heads whose product with it is minus infinity do not see the row; the others have no number, nor have the sums that they add to."""
+    c = Cache(SHAPES[shape], 2, d, 16, dtype)
+    for b in range(0, len(c.lens), 2):
+        _row(c, c.k, b, (b * 11) % c.lens[b])[1, 6] = bad
+    _check(c, 8, weights=True)
+
+
+@pytest.mark.parametrize("lens", [[1], [40], [700], [9000]])
+def test_rows_that_are_all_minus_infinity(lens):
+    """0 / 0: the softmax of nothing but minus infinities is no number.  A sequence without rows has zeros."""
+    c = Cache(lens + [0, 3], 2, 64, 16, BF)
+    q = c.queries(4).abs()
+    for j in range(0, lens[0], 16):
+        c.k[int(c.table[0, j // 16]), :, 1, 0] = -INF
+    value = _check(c, 4, weights=True, q=q)
+    assert value[0, 2:].isnan().all() and value[0, :2].isfinite().all() and (value[1] == 0).all()

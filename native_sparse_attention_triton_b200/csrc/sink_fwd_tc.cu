@@ -286,7 +286,8 @@ sink_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     }
     // ---- epilogue: O / sum, 64 columns at a time ----
     const float inv = l_rounded > 0.f ? 1.f / l_rounded : 0.f, lse = m_ref + log2f(l);
-    if (valid) p.lse[(long long)(qs + tpos) * p.Hq + head] = l > 0.f ? lse : -INFINITY;
+    // (of a row whose sum is no number none either: with minus infinity the backward pass would give its keys infinities)
+    if (valid) p.lse[(long long)(qs + tpos) * p.Hq + head] = l == 0.f ? -INFINITY : lse;
     // A row tile whose tokens all belong to the sequence leaves through the Q tile (free since the last S product, in the swizzled
     // panel layout) and one TMA store per panel; otherwise row by row.
     const bool staged = q0 + QT <= Lq;

@@ -285,9 +285,10 @@ sink_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       if (lane == 0) mbar_arrive(p_full + (i & 1));
     }
     // ---- epilogue: O / sum, 64 columns at a time ----
-    const float inv = l_rounded > 0.f ? 1.f / l_rounded : 0.f, lse = m_ref + log2f(l);
-    // (of a row whose sum is no number none either: with minus infinity the backward pass would give its keys infinities)
-    if (valid) p.lse[(long long)(qs + tpos) * p.Hq + head] = l == 0.f ? -INFINITY : lse;
+    // A query sees itself at least: its sum is zero where all its logits are minus infinity, and neither output nor log-sum-exp is a number then.
+    // (With minus infinity the backward pass would give its keys infinities, as for a sum that is none.)
+    const float inv = valid ? 1.f / l_rounded : 0.f, lse = l == 0.f ? NAN : m_ref + log2f(l);
+    if (valid) p.lse[(long long)(qs + tpos) * p.Hq + head] = lse;
     // A row tile whose tokens all belong to the sequence leaves through the Q tile (free since the last S product, in the swizzled
     // panel layout) and one TMA store per panel; otherwise row by row.
     const bool staged = q0 + QT <= Lq;

@@ -102,3 +102,20 @@ def test_many_key_heads_of_sixteen_queries(which):
         for name, g, val, t, hit in zip(("dq", "dk", "dv", "o"), got, (*value[1:], value[0]), (*bound[1:], bound[0]), touched):
             assert_within(g[~hit], val[~hit], t[~hit], name)
             assert g[hit].isnan().all(), name
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_rows_that_are_all_minus_infinity(graph):
+    """0 / 0: a query all of whose logits are minus infinity has no number, like those behind it that see such keys alone."""
+    from native_sparse_attention_triton_b200 import device_status, ops
+
+    lens = [1, 70, 200]
+    q, k, v, do = _inputs(lens, 4, 2, 128, BF, seed=7)
+    q.abs_()
+    k[0, 0, 3], k[1:30, 1, 4] = -INF, -INF
+    x = [t.requires_grad_(graph) for t in (q, k, v)]
+    o = ops.sink_window_attention(*x, _cu(lens), 10, 2).detach()
+    want = torch.zeros(271, 4, dtype=torch.bool, device="cuda")
+    want[0, :2], want[1:30, 2:] = True, True
+    assert torch.equal(o.isnan().all(-1), want) and torch.equal(o.isnan().any(-1), want)
+    assert device_status() == 0

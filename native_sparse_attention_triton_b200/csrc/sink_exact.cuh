@@ -8,6 +8,8 @@
 #include "common.cuh"
 #include "sink_keys.cuh"
 
+#include <cfloat>
+
 namespace nsa {
 
 // Elements lane * EPL .. of a row of D.
@@ -41,8 +43,10 @@ __device__ __noinline__ float4 exact_query_row(const SinkMaps* m, int row0, int 
   for (int j = gap_at > 0 ? 0 : first; j <= t; j = j + 1 == gap_at ? first : j + 1) {
     lane_elements<T, D>(k, m->keys, (long long)(row0 + j) * m->k_sn + kvh * m->k_sh);
     lane_elements<T, D>(v, m->values, (long long)(row0 + j) * m->v_sn + kvh * m->v_sh);
-    float w = fast_exp2(fmaf(warp_dot(q, k), scale2, -lse));
+    const float x = fmaf(warp_dot(q, k), scale2, -lse);
+    float w = fast_exp2(x);
     if constexpr (GRAD) w *= (warp_dot(g, v) - delta) * sm_scale;
+    else if (w == 0.f && x > -INFINITY) w = FLT_MIN;  // no probability is zero: infinity times it is infinity
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, GRAD ? k[e] : v[e], acc[e]);
   }

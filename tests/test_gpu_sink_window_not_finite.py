@@ -119,3 +119,19 @@ def test_rows_that_are_all_minus_infinity(graph):
     want[0, :2], want[1:30, 2:] = True, True
     assert torch.equal(o.isnan().all(-1), want) and torch.equal(o.isnan().any(-1), want)
     assert device_status() == 0
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_value_whose_probability_is_far_below_the_smallest_float(graph):
+    """A probability is above zero, however small, so that infinity times it is infinity."""
+    from native_sparse_attention_triton_b200 import ops
+
+    n = 300
+    q, k, v, _ = _inputs([n], 4, 2, 128, BF, seed=9)
+    k[5] = -q[200, ::2]  # logits of about -130 for two heads of query 200
+    v[5, :, 7] = INF
+    x = [t.requires_grad_(graph) for t in (q, k, v)]
+    o = ops.sink_window_attention(*x, _cu([n]), 250, 1, 3.0 / math.sqrt(128)).detach()
+    p = torch.softmax(q.detach()[200, 0].double() @ k.detach()[:201, 0].double().T * 3.0 / math.sqrt(128), 0)
+    assert 0 < p[5] < 1e-50
+    assert o[200, :, 7].isposinf().all() and o[200, :, :7].isfinite().all()

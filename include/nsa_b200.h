@@ -226,7 +226,8 @@ int nsa_window_attn_bwd(const void* q, const void* k, const void* v, const void*
 
 /* Sliding window with sinks: query t of a sequence sees key j <= t iff t - j <= window_left or j < num_sinks.  No counterpart in the
  * reference.  Tensors, strides and lse convention as nsa_window_attn_fwd / nsa_window_attn_bwd, head_dim 64 or 128; no bound on the lengths
- * is needed.  Output, dq, dk and dv of rows behind the last sequence are zero.  o_rest: NULL, or total_len * num_q_heads * d 16-bit
+ * is needed.  Output, dq, dk and dv of rows behind the last sequence are zero; a sequence that ends behind the rows ends with them, one that
+ * starts outside of them is none, and either raises device status 2.  o_rest: NULL, or total_len * num_q_heads * d 16-bit
  * elements, 16-byte aligned, that the forward fills for the backward in an order of its own with what the rounding of o took away: with it
  * sum_d o dO is exact to 2^-17 (2^-22), which rows that look at few keys need.  Workspace: nsa_sink_window_attn_bwd_workspace bytes. */
 int nsa_sink_window_attn_fwd(const void* q, const void* k, const void* v, const int* cu_seqlens, void* o, void* o_rest, float* lse,

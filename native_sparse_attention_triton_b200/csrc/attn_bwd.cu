@@ -856,8 +856,9 @@ __global__ void __launch_bounds__(256) sink_finish_kernel(DkdvParams p, SummedRo
   }
   const float zero = (a.x + a.y + a.z + a.w) * 0.f + (b.x + b.y + b.z + b.w) * 0.f;
   if (__any_sync(0xffffffffu, zero != 0.f) && n < __ldg(p.cu_q + p.B)) {
-    const int s = find_sequence(p.cu_q, p.B, n), row0 = __ldg(p.cu_q + s);
-    exact_key_row<T, D>(a, b, &maps, p.ld, p.Hq, row0, __ldg(p.cu_q + s + 1) - row0, n - row0, h, p.G, p.left, p.sinks, p.scale2, p.sm_scale);
+    const int s = find_sequence(p.cu_q, p.B, n), row0 = __ldg(p.cu_q + s), end = min(__ldg(p.cu_q + s + 1), r.total);
+    if (row0 >= 0 && row0 <= n && n < end)
+      exact_key_row<T, D>(a, b, &maps, p.ld, p.Hq, row0, end - row0, n - row0, h, p.G, p.left, p.sinks, p.scale2, p.sm_scale);
   }
   store_lane_elements<T, D>(static_cast<T*>(dk) + n * dk_sn + h * dk_sh, a);
   store_lane_elements<T, D>(static_cast<T*>(dv) + n * dv_sn + h * dv_sh, b);

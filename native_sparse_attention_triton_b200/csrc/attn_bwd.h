@@ -41,7 +41,7 @@ struct SummedRows {
     }
     const int b = (int)(x / (tiles * 128)), at = (int)(x % (tiles * 128)), start = __ldg(cu + b);
     n = start + at;
-    return at < __ldg(cu + b + 1) - start;
+    return at < __ldg(cu + b + 1) - start && start >= 0 && n < total;
   }
 };
 

@@ -94,10 +94,11 @@ sink_dkdv_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     st = slot % st_tiles;
     slot /= st_tiles;
   } else if (warp == 0 && blockIdx.y == 0) {
-    zero_rows_behind<T, D>(out.dk, out.dk_sn, out.dk_sh, __ldg(p.cu_q + p.B), out.rows, slot, p.key_slots, h, 1);
-    zero_rows_behind<T, D>(out.dv, out.dv_sn, out.dv_sh, __ldg(p.cu_q + p.B), out.rows, slot, p.key_slots, h, 1);
+    const int end = end_of_rows(p.cu_q, p.B, out.rows, p.st);
+    zero_rows_behind<T, D>(out.dk, out.dk_sn, out.dk_sh, end, out.rows, slot, p.key_slots, h, 1);
+    zero_rows_behind<T, D>(out.dv, out.dv_sn, out.dv_sh, end, out.rows, slot, p.key_slots, h, 1);
   }
-  if (!find_row_tile(p.cu_q, p.B, far ? p.sink_log : 7, slot, b, qs, Lq, tile)) return;
+  if (!find_tile_of_rows(p.cu_q, p.B, out.rows, far ? p.sink_log : 7, slot, p.st, b, qs, Lq, tile)) return;
   const int kpos = (far ? st : tile) * KT, krow0 = qs + kpos;
   const int kvalid = min(KT, (far ? min(p.sinks, Lq) : Lq) - kpos);
   if (far) {

@@ -64,10 +64,10 @@ sink_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   }
   const int QT = 128 >> p.logG, h = blockIdx.y;
   wait_for_launch_before();
-  const int batch_end = __ldg(p.cu_q + p.B);
   int b, qs, Lq, qt;
-  const bool work = find_row_tile(p.cu_q, p.B, 7 - p.logG, gridDim.x - 1 - blockIdx.x, b, qs, Lq, qt);
-  if (warp == 0) zero_rows_behind<T, D>(p.dq, p.dq_sn, p.dq_sh, batch_end, p.rows, blockIdx.x, gridDim.x, h * p.G, p.G);
+  const bool work = find_tile_of_rows(p.cu_q, p.B, p.rows, 7 - p.logG, gridDim.x - 1 - blockIdx.x, p.st, b, qs, Lq, qt);
+  if (warp == 0)
+    zero_rows_behind<T, D>(p.dq, p.dq_sn, p.dq_sh, end_of_rows(p.cu_q, p.B, p.rows, p.st), p.rows, blockIdx.x, gridDim.x, h * p.G, p.G);
   if (warp < 8) {  // a warp a row
     for (long long x = (long long)blockIdx.x * 8 + warp; x < p.summed.count(); x += gridDim.x * 8ll) {
       int n;

@@ -83,10 +83,10 @@ sink_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   }
   const int QT = 128 >> p.logG, h = blockIdx.y;
   wait_for_launch_before();
-  const int batch_end = __ldg(p.cu + p.B);
   int b, qs, Lq, qt;
-  const bool work = find_row_tile(p.cu, p.B, 7 - p.logG, gridDim.x - 1 - blockIdx.x, b, qs, Lq, qt);  // long rows first
-  if (warp == 0) zero_rows_behind<T, D>(p.o, p.o_sn, p.o_sh, batch_end, p.rows, blockIdx.x, gridDim.x, h * p.G, p.G);
+  const bool work = find_tile_of_rows(p.cu, p.B, p.rows, 7 - p.logG, gridDim.x - 1 - blockIdx.x, p.st, b, qs, Lq, qt);  // long rows first
+  if (warp == 0)
+    zero_rows_behind<T, D>(p.o, p.o_sn, p.o_sh, end_of_rows(p.cu, p.B, p.rows, p.st), p.rows, blockIdx.x, gridDim.x, h * p.G, p.G);
   if (!work) return;
   const int q0 = qt * QT;
   const int room = sink_room(p.sinks), shift = sink_shift(q0, p.left, room);

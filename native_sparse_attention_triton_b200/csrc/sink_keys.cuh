@@ -9,6 +9,7 @@
 // every row where there is a gap (their keys lie in front of the window), and are ordinary keys where there is none.
 #pragma once
 #include "tc5.cuh"
+#include "work_steal.cuh"
 
 namespace nsa {
 
@@ -59,6 +60,24 @@ __device__ __forceinline__ void clean_key_tile(uint32_t tile, int i, int n) {
 // two all but cancel, and what is left of o's rounding becomes as large as dS (one key of weight 1 - w: dS is w of its parts).
 __device__ __forceinline__ long long rest_chunk(int c, int kvh, int Hkv, int rows, int n, int G, int g) {
   return (((long long)c * Hkv + kvh) * rows + n) * G + g;
+}
+
+// A row tile (find_row_tile) of a batch of `rows` rows.  What cu says is held against the rows there are: a tile outside of them is none, a sequence
+// that ends behind them ends with them, and either raises the status.  A whole warp.
+__device__ __forceinline__ bool find_tile_of_rows(const int* cu, int nseq, int rows, int log_per, int want, const Status& st, int& b, int& start,
+                                                  int& len, int& tile) {
+  if (!find_row_tile(cu, nseq, log_per, want, b, start, len, tile)) return false;
+  if (start >= 0 && tile >= 0 && len <= rows - start) return true;
+  if (lane_id() == 0) st.raise(kErrBadIndex);
+  if (start < 0 || start >= rows || tile < 0) return false;
+  len = min(len, rows - start);
+  return ((long long)tile << log_per) < len;
+}
+// The end of the last sequence, within the rows there are.
+__device__ __forceinline__ int end_of_rows(const int* cu, int nseq, int rows, const Status& st) {
+  const int end = __ldg(cu + nseq);
+  if ((end < 0 || end > rows || __ldg(cu) < 0) && lane_id() == 0) st.raise(kErrBadIndex);
+  return max(0, min(end, rows));
 }
 
 // Rows of G heads from `head` on that belong to no sequence (a padded batch), [first, rows), as zeros; block x of n takes every n-th.  A warp.

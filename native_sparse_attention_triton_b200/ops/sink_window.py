@@ -13,7 +13,8 @@ from .. import _lib
 def sink_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, window_size: int, num_sinks: int,
                           sm_scale: Optional[float] = None) -> torch.Tensor:
     """q [total, Hq, d], k/v [total, Hkv, d] (self-attention: one cu_seqlens, int32 [batch + 1]); key j of a sequence is visible to its
-    query i iff j <= i and (i - j <= window_size or j < num_sinks).
+    query i iff j <= i and (i - j <= window_size or j < num_sinks).  cu_seqlens ascends from 0; a sequence that ends behind the rows ends with them,
+    and one that starts outside of them is none (either sets device status 2).
 
     bfloat16 or float16, head_dim 64 or 128, Hq / Hkv a power of two of at most 16 (NotImplementedError otherwise).  Differentiable in q, k
     and v.  Rows behind the last sequence (a padded batch) may hold anything: they reach no other row, and their output and gradients are

@@ -564,7 +564,9 @@ Tensor sliding_window_attention(const Tensor& q, const Tensor& k, const Tensor& 
 void check_captured_edges(const torch::autograd::Node& node, const at::Device& device) {
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
   const c10::Stream outside = c10::cuda::getDefaultCUDAStream(device.index()).unwrap();
-  for (const auto& edge : node.next_edges()) {
+  for (size_t i = 0; i < node.num_outputs(); ++i) {
+    if (!node.task_should_compute_output(i)) continue;  // nobody asked for it: nothing is handed over
+    const auto& edge = node.next_edge(i);
     const auto stream = edge.function ? edge.function->stream() : std::nullopt;
     TORCH_CHECK(!stream || *stream != outside,
                 "an input of this captured backward pass belongs to a graph of the default stream that is still alive; "

@@ -216,6 +216,20 @@ Layout layout_of(SeqInfo& info, int ks, int st, const at::Device& device) {
 }
 
 // ----------------------------------------------------------------------------------------------------- autograd nodes
+// A backward pass that is being captured cannot hand a gradient to the default stream, which is where the gradient accumulator of a leaf runs that
+// has been part of a graph built there, for as long as that graph lives.  The engine would find out behind the node's back, which ends the process.
+void check_captured_edges(const Node& node) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  for (size_t i = 0; i < node.num_outputs(); ++i) {
+    if (!node.task_should_compute_output(i)) continue;  // nobody asked for it: nothing is handed over
+    const auto& edge = node.next_edge(i);
+    const auto stream = edge.function ? edge.function->stream() : std::nullopt;
+    TORCH_CHECK(!stream || *stream != c10::cuda::getDefaultCUDAStream(stream->device_index()).unwrap(),
+                "an input of this captured backward pass belongs to a graph of the default stream that is still alive; "
+                "free that graph (or build it on the capturing stream) first");
+  }
+}
+
 // Saved tensors behind one lock, freed with the graph like those of torch's own nodes (a second backward without
 // retain_graph raises).  They are unpacked with autograd's dispatch keys in place: an unpack hook may run operators that have to be
 // recorded (activation checkpointing computes the forward again in there).
@@ -226,6 +240,7 @@ struct SavingNode : Node {
     for (auto& s : saved) s.reset_data();
   }
   std::vector<Tensor> unpack() {
+    check_captured_edges(*this);
     std::vector<Tensor> out;
     out.reserve(saved.size());
     for (auto& s : saved) out.push_back(s.unpack(shared_from_this()));
@@ -559,21 +574,6 @@ Tensor sliding_window_attention(const Tensor& q, const Tensor& k, const Tensor& 
 }
 
 // ----------------------------------------------------------------------------------------- sliding window with sinks
-// A backward pass that is being captured cannot hand a gradient to the default stream, which is where the gradient accumulator of a leaf runs that
-// has been part of a graph built there, for as long as that graph lives.  The engine would find out behind this node's back.
-void check_captured_edges(const torch::autograd::Node& node, const at::Device& device) {
-  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
-  const c10::Stream outside = c10::cuda::getDefaultCUDAStream(device.index()).unwrap();
-  for (size_t i = 0; i < node.num_outputs(); ++i) {
-    if (!node.task_should_compute_output(i)) continue;  // nobody asked for it: nothing is handed over
-    const auto& edge = node.next_edge(i);
-    const auto stream = edge.function ? edge.function->stream() : std::nullopt;
-    TORCH_CHECK(!stream || *stream != outside,
-                "an input of this captured backward pass belongs to a graph of the default stream that is still alive; "
-                "free that graph (or build it on the capturing stream) first");
-  }
-}
-
 struct SinkWindowBackward final : SavingNode {
   int left, sinks;
   double scale;
@@ -588,7 +588,6 @@ struct SinkWindowBackward final : SavingNode {
     const int64_t N = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = k.size(1);
     for (int i = 0; i < 3; ++i) out[i] = empty_like_rows(s[i]);
     if (N == 0) return out;
-    check_captured_edges(*this, q.device());
     const Tensor dout = gradient_rows(grads[0]);
     const long long bytes = nsa_sink_window_attn_bwd_workspace((int)N, (int)Hq, (int)Hkv, (int)D);
     Tensor ws = empty({bytes}, at::kByte, q.device());

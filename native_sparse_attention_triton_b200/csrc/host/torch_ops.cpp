@@ -97,17 +97,12 @@ Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const at::Device& devic
 }
 Tensor empty_like_rows(const Tensor& t) { return empty(t.sizes(), t.scalar_type(), t.device()); }
 
-// Kernels need a unit innermost stride and 16-byte aligned rows; copied only when that does not hold.
+// Kernels need a unit innermost stride and 16-byte aligned rows; copied only when that does not hold (a contiguous view at an odd offset, and one
+// row with an odd stride, are copied too, which contiguous() would return as they are).
 Tensor inner_contiguous(const Tensor& t) {
   bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   for (int64_t i = 0; ok && i + 1 < t.dim(); ++i) ok = t.stride(i) % 8 == 0;
-  return ok ? t : t.contiguous();
-}
-
-// An output gradient as the kernels read it: also copied where it is a contiguous view at an odd offset.
-Tensor gradient_rows(const Tensor& t) {
-  const Tensor rows = inner_contiguous(t);
-  return reinterpret_cast<uintptr_t>(rows.data_ptr()) % 16 ? rows.clone() : rows;
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 // The tensors' device made current, and its current stream.
@@ -299,7 +294,7 @@ struct CompressBackward final : SavingNode {
     at::AutoDispatchBelowADInplaceOrView guard;
     const Tensor &x = s[0], &w = s[1], &pe = s[2], &cu = s[3], &ycu = s[4];
     const int64_t N = x.size(0), H = x.size(1), D = x.size(2);
-    const Tensor dy = gradient_rows(grads[0].contiguous());
+    const Tensor dy = inner_contiguous(grads[0].contiguous());
     Tensor dx = empty({N, H, D}, x.scalar_type(), x.device()), dw, dpe;
     if (has_w) dw = empty(w.sizes(), w.scalar_type(), w.device());
     if (has_pe) dpe = empty(pe.sizes(), pe.scalar_type(), pe.device());
@@ -453,7 +448,7 @@ struct DenseAttentionBackward final : SavingNode {
       out = {dq.zero_(), dk, dv};
       return out;
     }
-    const Tensor dout = gradient_rows(grads[0]);
+    const Tensor dout = inner_contiguous(grads[0]);
     const int batch = (int)cu_q.size(0) - 1;
     const long long least = nsa_varlen_attn_bwd_workspace((int)N, (int)Nk, (int)Hq, (int)Hkv, (int)D);
     // one pass adds dQ up in the order in which CTAs arrive, the dQ pass in a fixed one
@@ -588,7 +583,7 @@ struct SinkWindowBackward final : SavingNode {
     const int64_t N = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = k.size(1);
     for (int i = 0; i < 3; ++i) out[i] = empty_like_rows(s[i]);
     if (N == 0) return out;
-    const Tensor dout = gradient_rows(grads[0]);
+    const Tensor dout = inner_contiguous(grads[0]);
     const long long bytes = nsa_sink_window_attn_bwd_workspace((int)N, (int)Hq, (int)Hkv, (int)D);
     Tensor ws = empty({bytes}, at::kByte, q.device());
     QkvStrides st;
@@ -669,7 +664,7 @@ struct SparseAttentionBackward final : SavingNode {
     const int batch = (int)cu.size(0) - 1;
     Tensor dq = empty({N, Hq, D}, q.scalar_type(), q.device()), dk = empty({N, Hkv, D}, q.scalar_type(), q.device()),
            dv = empty({N, Hkv, D}, q.scalar_type(), q.device());
-    const Tensor dout = gradient_rows(grads[0]);
+    const Tensor dout = inner_contiguous(grads[0]);
     const long long bytes = nsa_topk_sparse_attn_bwd_workspace((int)N, batch, (int)Hq, (int)Hkv, (int)D, (int)topk, block_size);
     Tensor ws = empty({std::max<long long>(bytes, 16)}, at::kByte, q.device());
     QkvStrides st;
@@ -740,7 +735,7 @@ struct GateCombineBackward final : SavingNode {
     const auto s = unpack();
     at::AutoDispatchBelowADInplaceOrView guard;
     const Tensor& gate = s[0];
-    const Tensor dout = gradient_rows(grads[0]);
+    const Tensor dout = inner_contiguous(grads[0]);
     for (int i = 0; i < 4; ++i) out[i] = empty_like_rows(s[i]);
     QkvStrides st;
     st.add(gate).add(s[1]).add(s[2]).add(s[3]).add(dout).add(out[0]).add(out[1]).add(out[2]).add(out[3]);
@@ -813,7 +808,7 @@ struct RopeBackward final : SavingNode {
     if (!grads[0].defined()) return out;
     const auto s = unpack();
     at::AutoDispatchBelowADInplaceOrView guard;
-    out[0] = rope_launch(gradient_rows(grads[0]), s[0], s[1], m, 1);
+    out[0] = rope_launch(inner_contiguous(grads[0]), s[0], s[1], m, 1);
     return out;
   }
 };

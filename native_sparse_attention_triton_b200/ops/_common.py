@@ -27,6 +27,7 @@ def require_cuda(*tensors):
 
 
 def inner_contiguous(t: torch.Tensor) -> torch.Tensor:
-    """Kernels need a unit innermost stride, 16-byte aligned rows; copy only when that does not hold."""
+    """Kernels need a unit innermost stride, 16-byte aligned rows; copy only when that does not hold (contiguous() would return a contiguous view
+    at an odd offset, and one row with an odd stride, as they are)."""
     ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1])
-    return t if ok else t.contiguous()
+    return t if ok else t.clone(memory_format=torch.contiguous_format)

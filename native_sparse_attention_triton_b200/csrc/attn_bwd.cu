@@ -847,16 +847,16 @@ __global__ void __launch_bounds__(256) sink_finish_kernel(DkdvParams p, SummedRo
   x = (long long)n * p.Hkv + h;
   float4 a, b;
   if constexpr (D == 128) {
-    a = __ldcs(reinterpret_cast<const float4*>(p.dk32 + x * D) + lane);
-    b = __ldcs(reinterpret_cast<const float4*>(p.dv32 + x * D) + lane);
+    a = load_fresh<kOnce>(reinterpret_cast<const float4*>(p.dk32 + x * D) + lane);
+    b = load_fresh<kOnce>(reinterpret_cast<const float4*>(p.dv32 + x * D) + lane);
   } else {
-    const float2 a2 = __ldcs(reinterpret_cast<const float2*>(p.dk32 + x * D) + lane), b2 = __ldcs(reinterpret_cast<const float2*>(p.dv32 + x * D) + lane);
+    const float2 a2 = load_fresh<kOnce>(reinterpret_cast<const float2*>(p.dk32 + x * D) + lane), b2 = load_fresh<kOnce>(reinterpret_cast<const float2*>(p.dv32 + x * D) + lane);
     a = make_float4(a2.x, a2.y, 0.f, 0.f);
     b = make_float4(b2.x, b2.y, 0.f, 0.f);
   }
   const float zero = (a.x + a.y + a.z + a.w) * 0.f + (b.x + b.y + b.z + b.w) * 0.f;
-  if (__any_sync(0xffffffffu, zero != 0.f) && n < __ldg(p.cu_q + p.B)) {
-    const int s = find_sequence(p.cu_q, p.B, n), row0 = __ldg(p.cu_q + s), end = min(__ldg(p.cu_q + s + 1), r.total);
+  if (__any_sync(0xffffffffu, zero != 0.f) && n < load_fresh(p.cu_q + p.B)) {
+    const int s = find_sequence(p.cu_q, p.B, n), row0 = load_fresh(p.cu_q + s), end = min(load_fresh(p.cu_q + s + 1), r.total);
     if (row0 >= 0 && row0 <= n && n < end)
       exact_key_row<T, D>(a, b, &maps, p.ld, p.Hq, row0, end - row0, n - row0, h, p.G, p.left, p.sinks, p.scale2, p.sm_scale);
   }

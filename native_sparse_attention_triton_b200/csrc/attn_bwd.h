@@ -37,11 +37,11 @@ struct SummedRows {
   __device__ __forceinline__ bool row(long long x, int& n) const {
     if (!by_sequence()) {
       n = (int)x;
-      return tiles < 0 || (n < __ldg(cu + B) && n - __ldg(cu + find_sequence(cu, B, n)) < tiles * 128);
+      return tiles < 0 || (n < load_fresh(cu + B) && n - load_fresh(cu + find_sequence(cu, B, n)) < tiles * 128);
     }
-    const int b = (int)(x / (tiles * 128)), at = (int)(x % (tiles * 128)), start = __ldg(cu + b);
+    const int b = (int)(x / (tiles * 128)), at = (int)(x % (tiles * 128)), start = load_fresh(cu + b);
     n = start + at;
-    return at < __ldg(cu + b + 1) - start && start >= 0 && n < total;
+    return at < load_fresh(cu + b + 1) - start && start >= 0 && n < total;
   }
 };
 

@@ -60,19 +60,24 @@ __device__ __forceinline__ void load_a_frags(uint32_t (&a)[KS][4], uint32_t tile
 }
 
 // A-operand fragments of a 16-row tile read straight from global memory.
-// rowptr(r) returns the address of row r (r in 0..15) or nullptr for a padding row.
-template <typename T, int KS, typename RowPtr>
+// rowptr(r) returns the address of row r (r in 0..15) or nullptr for a padding row.  FRESH: in a kernel that is launched early (load_fresh).
+template <typename T, int KS, bool FRESH = false, typename RowPtr>
 __device__ __forceinline__ void load_a_frags_global(uint32_t (&a)[KS][4], RowPtr rowptr) {
   const int l = lane_id();
   const T* r0 = rowptr(l >> 2);
   const T* r1 = rowptr((l >> 2) + 8);
   const int c = (l & 3) * 2;
+  const auto load = [](const T* p) {
+    const uint32_t* u = reinterpret_cast<const uint32_t*>(p);
+    if constexpr (FRESH) return load_fresh(u);
+    else return __ldg(u);
+  };
 #pragma unroll
   for (int kk = 0; kk < KS; ++kk) {
-    a[kk][0] = r0 ? __ldg(reinterpret_cast<const uint32_t*>(r0 + kk * 16 + c)) : 0u;
-    a[kk][1] = r1 ? __ldg(reinterpret_cast<const uint32_t*>(r1 + kk * 16 + c)) : 0u;
-    a[kk][2] = r0 ? __ldg(reinterpret_cast<const uint32_t*>(r0 + kk * 16 + c + 8)) : 0u;
-    a[kk][3] = r1 ? __ldg(reinterpret_cast<const uint32_t*>(r1 + kk * 16 + c + 8)) : 0u;
+    a[kk][0] = r0 ? load(r0 + kk * 16 + c) : 0u;
+    a[kk][1] = r1 ? load(r1 + kk * 16 + c) : 0u;
+    a[kk][2] = r0 ? load(r0 + kk * 16 + c + 8) : 0u;
+    a[kk][3] = r1 ? load(r1 + kk * 16 + c + 8) : 0u;
   }
 }
 

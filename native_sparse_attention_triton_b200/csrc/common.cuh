@@ -147,14 +147,38 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
 // In a kernel that was launched early (host_util.h): the kernel in front of it has finished and its writes are visible.
 __device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 
+// Loads behind that wait, of what a kernel in front may have written: any input.  __ldg is for data that nobody writes while the kernel lives, which
+// begins before the wait, and a compiler may move it (and the other load intrinsics, which are not volatile) in front of the wait.  kOnce: nobody reads
+// the data again; kShared: another SM wrote it in this kernel.
+enum LoadHint { kCached, kOnce, kShared };
+template <LoadHint HINT = kCached, typename T>
+__device__ __forceinline__ T load_fresh(const T* p) {
+  static_assert(sizeof(T) == 4 || sizeof(T) == 8 || sizeof(T) == 16, "32, 64 or 128 bits");
+  T x;
+  uint32_t* u = reinterpret_cast<uint32_t*>(&x);
+#define NSA_LOAD(HOW)                                                                                                                     \
+  if constexpr (sizeof(T) == 4) asm volatile("ld.global" HOW ".b32 %0, [%1];\n" : "=r"(u[0]) : "l"(p));                                    \
+  else if constexpr (sizeof(T) == 8) asm volatile("ld.global" HOW ".v2.b32 {%0, %1}, [%2];\n" : "=r"(u[0]), "=r"(u[1]) : "l"(p));          \
+  else asm volatile("ld.global" HOW ".v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]) : "l"(p))
+  if constexpr (HINT == kOnce) {
+    NSA_LOAD(".cs");
+  } else if constexpr (HINT == kShared) {
+    NSA_LOAD(".cg");
+  } else {
+    NSA_LOAD("");
+  }
+#undef NSA_LOAD
+  return x;
+}
+
 __device__ __forceinline__ int lane_id() { return threadIdx.x & 31; }
 
 // largest b such that cu[b] <= n (cu has nseq+1 ascending entries, cu[0] = 0)
-__device__ __forceinline__ int find_sequence(const int* __restrict__ cu, int nseq, int n) {
+__device__ __forceinline__ int find_sequence(const int* cu, int nseq, int n) {
   int lo = 0, hi = nseq;  // invariant: cu[lo] <= n < cu[hi]
   while (hi - lo > 1) {
     int mid = (lo + hi) >> 1;
-    if (__ldg(cu + mid) <= n) lo = mid; else hi = mid;
+    if (load_fresh(cu + mid) <= n) lo = mid; else hi = mid;
   }
   return lo;
 }

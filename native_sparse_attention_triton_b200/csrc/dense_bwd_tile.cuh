@@ -13,14 +13,17 @@ __device__ __forceinline__ void red_add_v4(float* dst, const uint32_t* v) {
 
 // -lse (base 2) and delta * sm_scale of a tile's 128 rows, four a lane; rows past the last token have probability 0.
 __device__ __forceinline__ void fill_row_table(float* nlse, float* dsc, const DkdvParams& p, int logG, int h, int qs, int tok0, int tok_end, int lane) {
+  float2 ldv[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int r = lane + 32 * j;
-    const int tok = tok0 + (r >> logG);
-    float2 ldv = make_float2(INFINITY, 0.f);
-    if (tok < tok_end) ldv = __ldg(p.ld + (long long)(qs + tok) * p.Hq + h * p.G + (r & (p.G - 1)));
-    nlse[r] = -ldv.x;
-    dsc[r] = ldv.y * p.sm_scale;
+    const int r = lane + 32 * j, tok = tok0 + (r >> logG);
+    ldv[j] = make_float2(INFINITY, 0.f);
+    if (tok < tok_end) ldv[j] = load_fresh(p.ld + (long long)(qs + tok) * p.Hq + h * p.G + (r & (p.G - 1)));
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    nlse[lane + 32 * j] = -ldv[j].x;
+    dsc[lane + 32 * j] = ldv[j].y * p.sm_scale;
   }
 }
 

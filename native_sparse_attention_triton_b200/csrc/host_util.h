@@ -57,7 +57,7 @@ struct LaunchScope {
 };
 
 // A launch whose CTAs may be set up while the kernel in front of it in the stream still runs (programmatic dependent launch).  The kernel has to
-// call wait_for_launch_before() (common.cuh) before it touches memory.
+// call wait_for_launch_before() (common.cuh) before it touches memory, and to load by load_fresh or TMA, or through plain pointers that are not __restrict__.
 template <typename... P, typename... A>
 cudaError_t launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
   cudaLaunchAttribute early;

@@ -40,12 +40,12 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedAppendParams p) 
   const int lane = lane_id();
   wait_for_launch_before();
   for (int b = blockIdx.x * 256 + threadIdx.x; b < p.B; b += gridDim.x * 256)
-    p.after[b] = min(p.cap, __ldg(p.held + b) + (p.cu ? __ldg(p.cu + b + 1) - __ldg(p.cu + b) : 1));
+    p.after[b] = min(p.cap, load_fresh(p.held + b) + (p.cu ? load_fresh(p.cu + b + 1) - load_fresh(p.cu + b) : 1));
   const int n = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (n >= (p.cu ? min(p.N, __ldg(p.cu + p.B)) : p.N)) return;  // rows behind the last sequence are nobody's
+  if (n >= (p.cu ? min(p.N, load_fresh(p.cu + p.B)) : p.N)) return;  // rows behind the last sequence are nobody's
   const int b = p.cu ? find_sequence(p.cu, p.B, n) : n;
-  const int pos = __ldg(p.held + b) + (p.cu ? n - __ldg(p.cu + b) : 0);
-  const int pg = pos >= 0 && pos < p.cap ? __ldg(p.table + b * p.t_sb + pos / p.page) : -1;
+  const int pos = load_fresh(p.held + b) + (p.cu ? n - load_fresh(p.cu + b) : 0);
+  const int pg = pos >= 0 && pos < p.cap ? load_fresh(p.table + b * p.t_sb + pos / p.page) : -1;
   if ((unsigned)pg >= (unsigned)p.num_pages) {
     if (lane == 0) p.st.raise(kErrBadIndex);
     return;
@@ -62,8 +62,8 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedAppendParams p) 
     for (int x = 0; x < 4; ++x) {
       const int c = c0 + 32 * x, h = c / CH, e = c % CH * 8;
       if (c < chunks) {
-        kr[x] = __ldg(reinterpret_cast<const uint4*>(k + h * p.k_sh + e));
-        vr[x] = __ldg(reinterpret_cast<const uint4*>(v + h * p.v_sh + e));
+        kr[x] = load_fresh(reinterpret_cast<const uint4*>(k + h * p.k_sh + e));
+        vr[x] = load_fresh(reinterpret_cast<const uint4*>(v + h * p.v_sh + e));
       }
     }
 #pragma unroll
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(PagedEvict
   __shared__ uint32_t s_digit, s_rank;
   const int b = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv, tid = threadIdx.x;
   wait_for_launch_before();
-  const int len = __ldg(p.seqlens + b), L = max(0, min(len, p.cap)), m = min(L, p.budget);
+  const int len = load_fresh(p.seqlens + b), L = max(0, min(len, p.cap)), m = min(L, p.budget);
   if (len > p.cap && tid == 0) p.st.raise(kErrBadIndex);
   const float* w = p.w + b * p.w_sb + h * p.w_sh;
   float* w_out = p.w_out + (long long)blockIdx.x * p.w_cols;
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(PagedEvict
   if (L <= p.budget) {
     for (int i = tid; i < m; i += kSelectThreads) {
       kept[i] = i;
-      w_out[i] = __ldg(w + i);
+      w_out[i] = load_fresh(w + i);
     }
     return;
   }
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(PagedEvict
     for (int j = 0; j < kSelectItems; ++j) {
       const int i = base + first + 32 * j;
       const bool in = j < per && i < L;
-      x[j] = in ? __ldg(w + i) : 0.f;
+      x[j] = in ? load_fresh(w + i) : 0.f;
       within |= (in ? 1u : 0u) << j;
       between |= (in && i >= lo && i < hi ? 1u : 0u) << j;
     }
@@ -253,14 +253,14 @@ __global__ void __launch_bounds__(256) evict_move_kernel(PagedEvictParams p) {
   constexpr int CH = D / 8, AT_ONCE = 32 / (2 * CH);  // rows copied by one step
   wait_for_launch_before();
   const int b = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv, lane = lane_id();
-  const int m = min(max(0, min(__ldg(p.seqlens + b), p.cap)), p.budget);
+  const int m = min(max(0, min(load_fresh(p.seqlens + b), p.cap)), p.budget);
   const int i0 = (blockIdx.y * 8 + (threadIdx.x >> 5)) * 16;
   if (i0 >= m) return;
   int from = -1, to = -1, from_slot = 0, to_slot = 0;
   if (lane < 16 && i0 + lane < m) {
-    const int i = i0 + lane, j = __ldg(p.kept + (long long)blockIdx.x * p.budget + i);
-    from = __ldg(p.table + b * p.t_sb + j / p.page);
-    to = __ldg(p.target + b * p.n_sb + i / p.page);
+    const int i = i0 + lane, j = load_fresh(p.kept + (long long)blockIdx.x * p.budget + i);
+    from = load_fresh(p.table + b * p.t_sb + j / p.page);
+    to = load_fresh(p.target + b * p.n_sb + i / p.page);
     from_slot = j % p.page;
     to_slot = i % p.page;
     if ((unsigned)from >= (unsigned)p.num_pages || (unsigned)to >= (unsigned)p.num_pages) {
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(256) evict_move_kernel(PagedEvictParams p) {
       const int f = __shfl_sync(0xffffffffu, from, row), fs = __shfl_sync(0xffffffffu, from_slot, row);
       const int t = __shfl_sync(0xffffffffu, to, row), ts = __shfl_sync(0xffffffffu, to_slot, row);
       dst[x] = t < 0 ? -1 : t * sp + ts * ss;
-      if (t >= 0) r[x] = __ldcs(reinterpret_cast<const uint4*>(base + f * sp + fs * ss));
+      if (t >= 0) r[x] = load_fresh<kOnce>(reinterpret_cast<const uint4*>(base + f * sp + fs * ss));
     }
 #pragma unroll
     for (int x = 0; x < 8; ++x)

@@ -71,7 +71,7 @@ struct Rows {
 __device__ __forceinline__ Rows visible_rows(const PagedDecodeParams& p, int b) {
   constexpr int R = kPagedRows;
   Rows r;
-  r.len = max(0, min(__ldg(p.seqlens + b), p.cap));
+  r.len = max(0, min(load_fresh(p.seqlens + b), p.cap));
   r.first = p.window < 0 ? 0 : max(0, r.len - 1 - p.window);
   r.head = min(p.sinks, r.first);
   r.gap_at = min((r.head + R - 1) / R, r.first / R);
@@ -101,7 +101,7 @@ __device__ __forceinline__ unsigned count_tiles(const PagedDecodeParams& p, unsi
   unsigned sum = 0;
   for (int b = b0; b < b1; ++b) {
     sum += visible_rows(p, b).n;
-    if (blockIdx.x == 0 && __ldg(p.seqlens + b) > p.cap) p.st.raise(kErrBadIndex);  // more rows than its pages hold
+    if (blockIdx.x == 0 && load_fresh(p.seqlens + b) > p.cap) p.st.raise(kErrBadIndex);  // more rows than its pages hold
   }
   sum *= p.Hkv;
   unsigned upto = sum;
@@ -200,7 +200,7 @@ __device__ __noinline__ void exact_decode_row(const PagedDecodeParams* p, int b,
   for (int t = 0; t < rows.n; ++t) {
     const int j = (t < rows.gap_at ? t : t + rows.gap) * kPagedRows + lane;
     const bool in = j < rows.len && (j >= rows.first || j < rows.head);
-    const int page = in ? __ldg(p->table + (long long)b * p->t_sb + j / p->page) : -1;
+    const int page = in ? load_fresh(p->table + (long long)b * p->t_sb + j / p->page) : -1;
     for (unsigned see = __ballot_sync(0xffffffffu, (unsigned)page < (unsigned)p->num_pages); see; see &= see - 1) {
       const int src = __ffs(see) - 1;
       const long long pg = __shfl_sync(0xffffffffu, page, src), slot = __shfl_sync(0xffffffffu, j % p->page, src);
@@ -281,7 +281,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       in = more && j < ld.rows.len && (j >= ld.rows.first || j < ld.rows.head);
       const int pg = in ? j / p.page : 0;
       slot = j - pg * p.page;
-      page_id = in ? __ldg(p.table + (long long)ld.b * p.t_sb + pg) : -1;
+      page_id = in ? load_fresh(p.table + (long long)ld.b * p.t_sb + pg) : -1;
     };
     auto fetch = [&](int i) {  // tile number i of the run into its stage
       const int s = i % kPagedStages;
@@ -355,7 +355,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       if (!TMA) cp_async_commit();
       if (fresh) {
         const T* qb = static_cast<const T*>(p.q) + (long long)cur.b * p.q_sb + (long long)cur.h * p.G * p.q_sh;
-        load_a_frags_global<T, D / 16>(qf, [&](int r) { return r < p.G ? qb + (long long)r * p.q_sh : (const T*)nullptr; });
+        load_a_frags_global<T, D / 16, /*FRESH=*/true>(qf, [&](int r) { return r < p.G ? qb + (long long)r * p.q_sh : (const T*)nullptr; });
 #pragma unroll
         for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
         m[0] = m[1] = -INFINITY;
@@ -629,8 +629,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 #pragma unroll
         for (int r = 0; r < RY; ++r) {
           const int g = min(warp * RY + r, p.G - 1);
-          ml[c][r] = __ldcg(reinterpret_cast<const float2*>(src + 16 * D + 2 * g));
-          o[c][r] = __ldcg(reinterpret_cast<const Cols*>(src + g * D + lane * EPL));
+          ml[c][r] = load_fresh<kShared>(reinterpret_cast<const float2*>(src + 16 * D + 2 * g));
+          o[c][r] = load_fresh<kShared>(reinterpret_cast<const Cols*>(src + g * D + lane * EPL));
         }
       }
 #pragma unroll
@@ -680,9 +680,9 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(PagedDecodeParams p,
     float ls[4], x[4][kWeightRows];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      ls[g] = g0 + g < p.G ? __ldg(lse + g0 + g) : -INFINITY;
+      ls[g] = g0 + g < p.G ? load_fresh(lse + g0 + g) : -INFINITY;
 #pragma unroll
-      for (int y = 0; y < kWeightRows; ++y) x[g][y] = in[y] && g0 + g < p.G ? __ldg(logits + (long long)(g0 + g) * p.logit_row + y * 256) : 0.f;
+      for (int y = 0; y < kWeightRows; ++y) x[g][y] = in[y] && g0 + g < p.G ? load_fresh(logits + (long long)(g0 + g) * p.logit_row + y * 256) : 0.f;
     }
 #pragma unroll
     for (int g = 0; g < 4; ++g)

@@ -211,7 +211,7 @@ sink_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const bool valid = tpos < Lq;
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     // ---- delta = sum_d o dO of this row, o with what its rounding took away; each of the two threads sums half of the row ----
-    const float lse2 = valid ? __ldg(p.lse + (long long)(qs + tpos) * p.Hq + head) : INFINITY;
+    const float lse2 = valid ? load_fresh(p.lse + (long long)(qs + tpos) * p.Hq + head) : INFINITY;
     float part = 0.f;
     {
       const uint4* orow = reinterpret_cast<const uint4*>(static_cast<const T*>(p.o) + (long long)(qs + tpos) * p.o_sn + (long long)head * p.o_sh);
@@ -219,8 +219,8 @@ sink_dq_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) {
         const int ci = half * (D / 16) + c;  // 16-byte chunk of the row
-        hi[c] = valid ? __ldg(orow + ci) : make_uint4(0, 0, 0, 0);
-        lo[c] = valid && p.rest ? __ldcs(p.rest + rest_chunk(ci, h, p.Hkv, p.rows, qs + tpos, p.G, row & (p.G - 1))) : make_uint4(0, 0, 0, 0);
+        hi[c] = valid ? load_fresh(orow + ci) : make_uint4(0, 0, 0, 0);
+        lo[c] = valid && p.rest ? load_fresh<kOnce>(p.rest + rest_chunk(ci, h, p.Hkv, p.rows, qs + tpos, p.G, row & (p.G - 1))) : make_uint4(0, 0, 0, 0);
       }
       mbar_wait(do_full, 0, p.st);
       const uint32_t d_addr = smem_u32(do_sm) + row * 128;

@@ -66,7 +66,7 @@ __device__ __noinline__ void exact_key_row(float4& dk, float4& dv, const SinkMap
       const int head = kvh * G + x;
       lane_elements<T, D>(q, m->q, (long long)(row0 + t) * m->q_sn + head * m->q_sh);
       lane_elements<T, D>(g, m->dout, (long long)(row0 + t) * m->do_sn + head * m->do_sh);
-      const float2 s = __ldg(ld + (long long)(row0 + t) * Hq + head);
+      const float2 s = load_fresh(ld + (long long)(row0 + t) * Hq + head);
       const float p = fast_exp2(fmaf(warp_dot(q, k), scale2, -s.x)), ds = p * (warp_dot(g, v) - s.y) * sm_scale;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {

@@ -75,8 +75,8 @@ __device__ __forceinline__ bool find_tile_of_rows(const int* cu, int nseq, int r
 }
 // The end of the last sequence, within the rows there are.
 __device__ __forceinline__ int end_of_rows(const int* cu, int nseq, int rows, const Status& st) {
-  const int end = __ldg(cu + nseq);
-  if ((end < 0 || end > rows || __ldg(cu) < 0) && lane_id() == 0) st.raise(kErrBadIndex);
+  const int end = load_fresh(cu + nseq);
+  if ((end < 0 || end > rows || load_fresh(cu) < 0) && lane_id() == 0) st.raise(kErrBadIndex);
   return max(0, min(end, rows));
 }
 

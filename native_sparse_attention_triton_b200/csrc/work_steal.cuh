@@ -94,7 +94,7 @@ __host__ __device__ __forceinline__ long long row_tile_slots(long long tokens, l
 // 32 a turn, made 4096 sequences of 16 tokens, 64q/4kv, causal, take 6020 us; with a search it is 770, with a CTA per item and the
 // sequence in the grid it was 1010.)
 // A whole warp looks up slot `want`; false for a slot without a tile.
-__device__ __forceinline__ bool find_row_tile(const int* __restrict__ cu, int nseq, int log_per, int want, int& b, int& start, int& len,
+__device__ __forceinline__ bool find_row_tile(const int* cu, int nseq, int log_per, int want, int& b, int& start, int& len,
                                               int& tile) {
   const int lane = lane_id();
   int span = nseq, first = 0, next = 0, src = 0;
@@ -104,8 +104,8 @@ __device__ __forceinline__ bool find_row_tile(const int* __restrict__ cu, int ns
     const int mine = b + lane * step;
     const bool in = lane * step < span;
     if (in) {
-      first = __ldg(cu + mine);
-      if (step == 1) next = __ldg(cu + mine + 1);
+      first = load_fresh(cu + mine);
+      if (step == 1) next = load_fresh(cu + mine + 1);
     }
     const unsigned hit = __ballot_sync(0xffffffffu, in && row_tile_slots(first, mine, log_per) <= want);
     if (!hit) return false;

@@ -422,6 +422,9 @@ int nsa_paged_kv_append(void* k_pages, void* v_pages, const int* block_table, co
  * strides[13]: q_b q_h | (page, slot, head) of k_pages, v_pages | o_b o_h | block_table row | weights_b weights_h. */
 long long nsa_paged_decode_control_words(void);
 long long nsa_paged_decode_scratch_floats(int batch, int num_q_heads, int head_dim, int capacity, int with_weights);
+/* The same where window_left and num_sinks are known: with weights, logits of the tiles of 32 rows that those reach into suffice. */
+long long nsa_paged_decode_window_scratch_floats(int batch, int num_q_heads, int head_dim, int capacity, int with_weights, int window_left,
+                                                 int num_sinks);
 int nsa_paged_attn_decode(const void* q, const void* k_pages, const void* v_pages, const int* block_table, const int* seqlens, void* o,
                           float* weights, float* scratch, long long scratch_floats, int batch, int num_q_heads, int num_kv_heads,
                           int head_dim, int num_pages, int page_size, int max_pages, int window_left, int num_sinks,

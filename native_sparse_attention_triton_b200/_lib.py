@@ -74,6 +74,7 @@ _SIZE_QUERIES = {
     "nsa_sink_window_attn_bwd_workspace": [_I, _I, _I, _I],
     "nsa_paged_decode_control_words": [],
     "nsa_paged_decode_scratch_floats": [_I, _I, _I, _I, _I],
+    "nsa_paged_decode_window_scratch_floats": [_I, _I, _I, _I, _I, _I, _I],
     "nsa_topk_sparse_attn_bwd_workspace": [_I, _I, _I, _I, _I, _I, _I],
     "nsa_launch_count": [],
     "nsa_flash_attn_decode_static_capacity": [],

@@ -857,14 +857,17 @@ uint64_t scratch_key(const at::Device& d, const c10::cuda::CUDAStream& s) {
   return (reinterpret_cast<uint64_t>(s.stream()) << 6) ^ (uint64_t)(d.index() & 63);
 }
 
+// `n` floats, the first `ctrl` zero
+Tensor fresh_scratch(long long ctrl, long long n, const at::Device& device) {
+  Tensor t = empty({n}, at::kFloat, device);
+  t.narrow(0, 0, ctrl).zero_();
+  return t;
+}
+
 // `pairs`: (sequence, KV head) pairs; `n`: floats
 Tensor take_scratch(long long pairs, long long n, const at::Device& device, uint64_t key) {
   const long long ctrl = (pairs + 1 + 63) / 64 * 64;
-  const auto fresh = [&] {
-    Tensor t = empty({n}, at::kFloat, device);
-    t.narrow(0, 0, ctrl).zero_();
-    return t;
-  };
+  const auto fresh = [&] { return fresh_scratch(ctrl, n, device); };
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return fresh();
   std::lock_guard<std::mutex> lk(g_scratch_mu);
   auto it = g_scratch.find(key);
@@ -1053,6 +1056,10 @@ Tensor paged_kv_append(const Tensor& kp, const Tensor& vp, const Tensor& table, 
   return after;
 }
 
+// Logits grow with the table's width, not with the rows that sequences hold: beyond 64 MiB their scratch is the call's own and goes back to the
+// allocator behind it, instead of being kept for the stream.  Clearing its control words costs such a call up to 1 us of 25 to 200.
+constexpr long long kKeptLogits = 16ll << 20;  // floats
+
 Tensor paged_attention_decode(const Tensor& q_in, const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& seqlens,
                               std::optional<double> sm_scale, std::optional<int64_t> window, int64_t sinks, const OptTensor& weights) {
   const Pages c = check_pages(kp, vp, table, seqlens);
@@ -1080,9 +1087,10 @@ Tensor paged_attention_decode(const Tensor& q_in, const Tensor& kp, const Tensor
                             o.stride(1), table.stride(0), weights ? weights->stride(0) : 0, weights ? weights->stride(1) : 0};
   const int left = window ? (int)std::min<int64_t>(*window, INT_MAX / 2) : -1, s = (int)std::min<int64_t>(sinks, INT_MAX / 2);
   Launch run(q);
-  const long long n = nsa_paged_decode_scratch_floats((int)c.batch, (int)q.size(1), (int)c.d, (int)c.capacity, weights.has_value());
+  const long long n = nsa_paged_decode_window_scratch_floats((int)c.batch, (int)q.size(1), (int)c.d, (int)c.capacity, weights.has_value(), left, s);
   const uint64_t key = scratch_key(q.device(), c10::cuda::getCurrentCUDAStream(q.device().index()));
-  const Tensor buf = take_scratch(nsa_paged_decode_control_words() - 1, n, q.device(), key);
+  const long long words = nsa_paged_decode_control_words();
+  const Tensor buf = n <= kKeptLogits ? take_scratch(words - 1, n, q.device(), key) : fresh_scratch(words, n, q.device());
   const int rc = nsa_paged_attn_decode(ptr(q), ptr(kp), ptr(vp), ptr<int>(table), ptr<int>(seqlens), ptr(o), weights ? ptr<float>(*weights) : nullptr,
                                        ptr<float>(buf), n, (int)c.batch, (int)q.size(1), (int)c.heads, (int)c.d, (int)c.pages, (int)c.page,
                                        (int)c.columns, left, s, st, (float)scale, dtype_code(q), run.stream);

@@ -51,13 +51,13 @@ struct PagedDecodeParams {
   void* o;
   const int* table;
   const int* seqlens;
-  float* logits;  // [pairs][G][logit_row] base-2 logits by row, or nullptr
+  float* logits;  // [pairs][G][logit_row] base-2 logits of a sequence's tiles, or nullptr
   float* lse;     // [pairs][G], with logits
   unsigned* ctrl;
   float* part;    // [CTAs][2][16][D + 2]
   long long q_sb, q_sh, k_sp, k_ss, k_sh, v_sp, v_ss, v_sh, o_sb, o_sh, t_sb;
   int B, Hkv, G, page, max_pages, num_pages, cap;
-  int logit_row;      // cap rounded up to whole tiles
+  int logit_row;      // rows of the tiles that a sequence may have
   int box;            // rows of a TMA box: they divide a page and a tile
   int window, sinks;  // window < 0: every row
   float scale2;
@@ -400,7 +400,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         for (int half = 0; half < 2; ++half) {
           const int g = (lane >> 2) + half * 8;
           if (g < p.G) {
-            float* dst = p.logits + (pair * p.G + g) * p.logit_row + cur.row0() + c0;
+            float* dst = p.logits + (pair * p.G + g) * p.logit_row + cur.t * kPagedRows + c0;
 #pragma unroll
             for (int j = 0; j < NT; ++j) *reinterpret_cast<float2*>(dst + j * 8) = make_float2(x[j][2 * half], x[j][2 * half + 1]);
           }
@@ -658,31 +658,36 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 }
 
 constexpr int kWeightRows = 2;  // of a thread
-// weights[b][h][j] += sum over the G heads of 2^(x_j - lse), row by row of the logits the attention kernel left.
+// weights[b][h][j] += sum over the G heads of 2^(x_j - lse), row by row of the logits the attention kernel left: place u of a sequence's tiles.
 __global__ void __launch_bounds__(256) paged_weights_kernel(PagedDecodeParams p, float* weights, long long w_sb, long long w_sh) {
   wait_for_launch_before();
   const int b = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv;
   const Rows rows = visible_rows(p, b);
+  if ((int)blockIdx.y * 256 * kWeightRows >= rows.n * kPagedRows) return;
   float* out = weights + b * w_sb + h * w_sh;
   const float* lse = p.lse + (long long)blockIdx.x * p.G;
-  const int j0 = blockIdx.y * (256 * kWeightRows) + threadIdx.x;
+  const int u0 = blockIdx.y * (256 * kWeightRows) + threadIdx.x;
   float sum[kWeightRows], old[kWeightRows];
+  int at[kWeightRows];
   bool in[kWeightRows];
 #pragma unroll
   for (int y = 0; y < kWeightRows; ++y) {
-    const int j = j0 + y * 256;
+    const int u = u0 + y * 256, j = at[y] = u + (u / kPagedRows < rows.gap_at ? 0 : rows.gap * kPagedRows);
     in[y] = j < rows.len && (j < rows.head || j >= rows.first);
     old[y] = in[y] ? out[j] : 0.f;
     sum[y] = 0.f;
   }
-  const float* logits = p.logits + (long long)blockIdx.x * p.G * p.logit_row + j0;
-  for (int g0 = 0; g0 < p.G; g0 += 4) {  // the loads of four heads in front of their first use
+  // The loads of four heads in front of their first use, of places that stand for no row too: no branch between them, and nothing is made of those.
+  const float* logits = p.logits + (long long)blockIdx.x * p.G * p.logit_row;
+  for (int g0 = 0; g0 < p.G; g0 += 4) {
     float ls[4], x[4][kWeightRows];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      ls[g] = g0 + g < p.G ? load_fresh(lse + g0 + g) : -INFINITY;
+      const int head = min(g0 + g, p.G - 1);
+      ls[g] = load_fresh(lse + head);
+      if (g0 + g >= p.G) ls[g] = -INFINITY;
 #pragma unroll
-      for (int y = 0; y < kWeightRows; ++y) x[g][y] = in[y] && g0 + g < p.G ? load_fresh(logits + (long long)(g0 + g) * p.logit_row + y * 256) : 0.f;
+      for (int y = 0; y < kWeightRows; ++y) x[g][y] = load_fresh(logits + (long long)head * p.logit_row + min(u0 + y * 256, p.logit_row - 1));
     }
 #pragma unroll
     for (int g = 0; g < 4; ++g)
@@ -691,7 +696,15 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(PagedDecodeParams p,
   }
 #pragma unroll
   for (int y = 0; y < kWeightRows; ++y)
-    if (in[y]) out[j0 + y * 256] = old[y] + sum[y];
+    if (in[y]) out[at[y]] = old[y] + sum[y];
+}
+
+// Rows of the tiles that a sequence may have: those of its pages, and with a window no more than the window and the sinks reach into.
+static long long most_logits(long long capacity, long long window, long long sinks) {
+  const long long all = (capacity + kPagedRows - 1) / kPagedRows;
+  // the window's rows begin anywhere in a tile
+  const long long seen = window < 0 ? all : (window + 1 + kPagedRows - 1) / kPagedRows + 1 + (sinks + kPagedRows - 1) / kPagedRows;
+  return std::max(1ll, std::min(all, seen)) * kPagedRows;
 }
 
 // One float of control per CTA, rounded up to whole lines; the parts behind them; with weights the logits and log-sum-exps.
@@ -722,15 +735,21 @@ static int launch_paged_decode(PagedDecodeParams p, float* weights, long long w_
   }
   if (e != cudaSuccess || !weights) return cuda_rc(e);
   LaunchScope ls_("paged_weights", stream);
-  return cuda_rc(launch_early(paged_weights_kernel, dim3(p.B * p.Hkv, (p.cap + 256 * kWeightRows - 1) / (256 * kWeightRows)), 256, 0, stream, p, weights, w_sb, w_sh));
+  return cuda_rc(launch_early(paged_weights_kernel, dim3(p.B * p.Hkv, (p.logit_row + 256 * kWeightRows - 1) / (256 * kWeightRows)), 256, 0, stream, p, weights, w_sb, w_sh));
 }
 
 }  // namespace nsa
 
 extern "C" long long nsa_paged_decode_control_words(void) { return nsa::paged_ctrl_floats(); }
 
+extern "C" long long nsa_paged_decode_window_scratch_floats(int batch, int num_q_heads, int head_dim, int capacity, int with_weights, int window_left,
+                                                            int num_sinks) {
+  const long long rows = with_weights ? nsa::most_logits(capacity, window_left, num_sinks) : 0;
+  return nsa::paged_ctrl_floats() + nsa::paged_part_floats(head_dim) + (with_weights ? (long long)batch * num_q_heads * (rows + 1) + 64 : 0);
+}
+
 extern "C" long long nsa_paged_decode_scratch_floats(int batch, int num_q_heads, int head_dim, int capacity, int with_weights) {
-  return nsa::paged_ctrl_floats() + nsa::paged_part_floats(head_dim) + (with_weights ? (long long)batch * num_q_heads * ((capacity + 31ll) / 32 * 32 + 1) + 64 : 0);
+  return nsa_paged_decode_window_scratch_floats(batch, num_q_heads, head_dim, capacity, with_weights, -1, 0);
 }
 
 extern "C" int nsa_paged_attn_decode(const void* q, const void* k_pages, const void* v_pages, const int* block_table, const int* seqlens, void* o,
@@ -745,19 +764,21 @@ extern "C" int nsa_paged_attn_decode(const void* q, const void* k_pages, const v
   // tiles are counted in 32 bits
   if (cap > (1ll << 30) || (long long)batch * num_kv_heads > (1ll << 30) || (double)batch * num_kv_heads * (cap + 31) >= 0x1p36) return kUnsupported;
   if (num_q_heads / num_kv_heads > 16) return kUnsupported;
-  if (weights && cap > 65535ll * 256 * kWeightRows) return kUnsupported;
+  const long long logit_row = most_logits(cap, window_left, num_sinks);
+  if (weights && logit_row > 65535ll * 256 * kWeightRows) return kUnsupported;
   // strides: q_b q_h  k_page k_slot k_h  v_page v_slot v_h  o_b o_h  table_b  weights_b weights_h
   for (int i = 0; i < 10; ++i)
     if (strides[i] % 8) return kInvalid;
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(o)) return kInvalid;
-  if (scratch_floats < nsa_paged_decode_scratch_floats(batch, num_q_heads, head_dim, (int)cap, weights != nullptr)) return kWorkspace;
+  if (scratch_floats < nsa_paged_decode_window_scratch_floats(batch, num_q_heads, head_dim, (int)cap, weights != nullptr, window_left, num_sinks))
+    return kWorkspace;
   PagedDecodeParams p;
   p.q = q; p.k = k_pages; p.v = v_pages; p.o = o; p.table = block_table; p.seqlens = seqlens;
   p.ctrl = reinterpret_cast<unsigned*>(scratch);
   p.part = scratch + paged_ctrl_floats();
   p.lse = weights ? p.part + paged_part_floats(head_dim) : nullptr;
   p.logits = weights ? p.lse + ((long long)batch * num_q_heads + 31) / 32 * 32 : nullptr;
-  p.logit_row = (int)((cap + kPagedRows - 1) / kPagedRows * kPagedRows);
+  p.logit_row = (int)logit_row;
   p.q_sb = strides[0]; p.q_sh = strides[1];
   p.k_sp = strides[2]; p.k_ss = strides[3]; p.k_sh = strides[4];
   p.v_sp = strides[5]; p.v_ss = strides[6]; p.v_sh = strides[7];

@@ -36,6 +36,8 @@ def paged_attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     seqlens[b] - 1 - j <= window_size, or j < num_sinks: what the query sees in sink_window_attention.  A sequence without rows gets zeros.
     weights float32 [batch, num_kv_heads, max_pages * page_size or more]: the probabilities that each visible row receives, summed over
     the query heads of its key/value head, are added in place (paged_kv_evict goes by them); other entries are left as they are.
+    They take scratch of 4 bytes for each query head and row of the table (with a window: for the rows that it and the sinks reach into), of which
+    up to 64 MiB a stream are kept for the next call.
     Values that are not finite reach what the definition makes depend on them: a head whose logits hold NaN has no output, and adds NaN to the
     weights of the rows it sees.  Not differentiable.
     """

@@ -1042,7 +1042,9 @@ Tensor paged_kv_append(const Tensor& kp, const Tensor& vp, const Tensor& table, 
   if (cu) one_device(kp, *cu);
   at::NoGradGuard no_grad;
   at::AutoDispatchBelowADInplaceOrView guard;
-  const Tensor k = inner_contiguous(k_in), v = inner_contiguous(v_in);
+  // rows of the cache itself are read before any of it is written
+  const auto apart = [&](const Tensor& t) { return t.is_alias_of(kp) || t.is_alias_of(vp) ? t.clone(at::MemoryFormat::Contiguous) : inner_contiguous(t); };
+  const Tensor k = apart(k_in), v = apart(v_in);
   Tensor after = empty({c.batch}, at::kInt, kp.device());
   if (c.batch == 0) return after;
   const long long st[11] = {k.stride(0), k.stride(1), v.stride(0), v.stride(1), kp.stride(0), kp.stride(1), kp.stride(2), vp.stride(0), vp.stride(1),

@@ -21,7 +21,8 @@ def paged_kv_append(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: t
     """Writes k, v [rows, num_kv_heads, head_dim] behind the seqlens[b] rows that each sequence holds: rows cu_seqlens[b] to
     cu_seqlens[b + 1] (a prompt), or one row per sequence without cu_seqlens (a decode step).
 
-    The pages are written in place and must be in block_table already, those that are written by one sequence alone.  Returns the lengths
+    The pages are written in place and must be in block_table already, those that are written by one sequence alone; k and v may be rows of the
+    cache itself, as they are before the call.  Returns the lengths
     after that, a new int32 [batch]; rows beyond max_pages * page_size are dropped (device status 2).
     """
     return _lib.host().paged_kv_append(k_pages, v_pages, block_table, seqlens, k, v, cu_seqlens)

@@ -40,12 +40,13 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedAppendParams p) 
   const int lane = lane_id();
   wait_for_launch_before();
   for (int b = blockIdx.x * 256 + threadIdx.x; b < p.B; b += gridDim.x * 256)
-    p.after[b] = min(p.cap, load_fresh(p.held + b) + (p.cu ? load_fresh(p.cu + b + 1) - load_fresh(p.cu + b) : 1));
+    p.after[b] = (int)min((long long)p.cap, (long long)load_fresh(p.held + b) + (p.cu ? (long long)load_fresh(p.cu + b + 1) - load_fresh(p.cu + b) : 1));
   const int n = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (n >= (p.cu ? min(p.N, load_fresh(p.cu + p.B)) : p.N)) return;  // rows behind the last sequence are nobody's
   const int b = p.cu ? find_sequence(p.cu, p.B, n) : n;
-  const int pos = load_fresh(p.held + b) + (p.cu ? n - load_fresh(p.cu + b) : 0);
-  const int pg = pos >= 0 && pos < p.cap ? load_fresh(p.table + b * p.t_sb + pos / p.page) : -1;
+  const long long at = (long long)load_fresh(p.held + b) + (p.cu ? n - load_fresh(p.cu + b) : 0);
+  const int pos = at >= 0 && at < p.cap ? (int)at : -1;
+  const int pg = pos >= 0 ? load_fresh(p.table + b * p.t_sb + pos / p.page) : -1;
   if ((unsigned)pg >= (unsigned)p.num_pages) {
     if (lane == 0) p.st.raise(kErrBadIndex);
     return;

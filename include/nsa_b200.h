@@ -229,7 +229,8 @@ int nsa_window_attn_bwd(const void* q, const void* k, const void* v, const void*
  * is needed.  Output, dq, dk and dv of rows behind the last sequence are zero; a sequence that ends behind the rows ends with them, one that
  * starts outside of them is none, and either raises device status 2.  o_rest: NULL, or total_len * num_q_heads * d 16-bit
  * elements, 16-byte aligned, that the forward fills for the backward in an order of its own with what the rounding of o took away: with it
- * sum_d o dO is exact to 2^-17 (2^-22), which rows that look at few keys need.  Workspace: nsa_sink_window_attn_bwd_workspace bytes. */
+ * o is known to 2^-16 of itself (fp16: 2^-22, and no better than 2^-25), which rows that look at few keys need.  (Where all rows of a tile see all its
+ * keys, a third of the forward's exponentials are good to 7.5e-5.)  lse is NaN for rows that have no number.  Workspace: nsa_sink_window_attn_bwd_workspace bytes. */
 int nsa_sink_window_attn_fwd(const void* q, const void* k, const void* v, const int* cu_seqlens, void* o, void* o_rest, float* lse,
                              int total_len, int batch, int num_q_heads, int num_kv_heads, int head_dim, int window_left, int num_sinks,
                              const long long* strides, float sm_scale, int dtype, void* stream);

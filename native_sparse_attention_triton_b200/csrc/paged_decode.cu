@@ -7,8 +7,8 @@
 // Row j lies in page table[b][j / page], slot j % page.
 //
 // What bounds it is HBM: 4 D bytes of K and V per visible row and KV head against 4 D G flops, which 16 x 8 x 16 products of one warp
-// (rows = the G query heads of a KV head) take with room to spare.  76 sequences of 1 to 8192 tokens, 32q/4kv, d = 128: 133 us, 5.5 TB/s (tiles
-// with cp.async instead of TMA boxes: 182); one of 517 rows 12.6 us, of 20 000 clocks 5000 until its tile is there, 6000 for it and the join in the
+// (rows = the G query heads of a KV head) take with room to spare.  76 sequences of 1 to 8192 tokens, 32q/4kv, d = 128: 137 us, 5.4 TB/s (tiles
+// with cp.async instead of TMA boxes: 182); one of 517 rows 13.4 us (12.8 without a look at whether what is written is finite), of 20 000 clocks 5000 until its tile is there, 6000 for it and the join in the
 // CTA, 8500 for the join between CTAs.
 //
 // A sequence's rows are cut into tiles of 32; those with a visible row, of all (sequence, KV head) pairs, form one list, which is

@@ -12,10 +12,10 @@
 // A row tile sees few keys (9 tiles of 64 at a window of 512), so what bounds the pass is a CTA's beginning and end and the chain of a tile's softmax.
 // Hence 96 KB of shared memory and 256 columns of tensor memory, so that two CTAs share an SM and one works while the other loads, waits or
 // stores; and two logit buffers, so that the products of a tile run under the softmax of the one before it.  64q/4kv, window 512, 4 sinks, 32 768
-// tokens, with o's rest and one part of P (below): 895 us; of a CTA's 22 600 clocks 4000 pass until its first logits, 900 and a hand-over of 300 a tile of
-// 64 (2200 the first, 1700 the last, which are masked), 4900 from the last P to the end.  Two threads per row made a tile's softmax no shorter
-// (920 us: the exponential unit then serves four warps); the dense forward's organisation (two row tiles in one CTA, tiles of 128 keys, one logit
-// buffer each, persistent) took 911 us without the rest and 1074 with it.
+// tokens: 775 us alone, 1050 in front of a backward pass (REST below).  Of the 22 600 clocks of a CTA that wrote o's rest with one part of P (895 us) 4000
+// passed until its first logits, 900 and a hand-over of 300 a tile of 64 (2200 the first, 1700 the last, which are masked), 4900 from the last P to the
+// end.  Against that variant two threads per row made a tile's softmax no shorter (920 us: the exponential unit then serves four warps); the dense
+// forward's organisation (two row tiles in one CTA, tiles of 128 keys, one logit buffer each, persistent) took 911 us without the rest and 1074 with it.
 #include <type_traits>
 
 #include "attn_tile.cuh"
@@ -51,7 +51,7 @@ struct SinkFwdParams {
 
 // REST: for a backward pass.  The probabilities are then two 16-bit parts, p = hi + lo, and P V two products: the backward pass needs sum_d o dO
 // next to single dO v, and one part's rounding in o (2^-9 of each p in bf16) would add to dS, which is rounded itself, more than half as much
-// again.  Packed 32 K tokens: 915 -> 1085 us; errors against 64 bits, in
+// again.  Packed 32 K tokens: 915 us with o's rest and one part, 1085 with two; errors against 64 bits, in
 // units of the final rounding: o 1.36 -> 1.00, dQ 1.50 -> 1.43, dK 1.46 -> 1.41 (1.41 is what rounding dS alone leaves).
 template <typename T, int D, bool REST>
 __global__ void __launch_bounds__(kThreads, 2)

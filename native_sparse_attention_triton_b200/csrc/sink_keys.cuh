@@ -55,7 +55,8 @@ __device__ __forceinline__ void clean_key_tile(uint32_t tile, int i, int n) {
   if (end < KEYS) zero_tile_rows<PANELS, KEYS * 128>(tile, max(0, end), KEYS);
 }
 
-// What the rounding of the output o took away, rounded itself (o is then known to 2^-17, or 2^-22 in fp16): 16-byte chunk c of a row, in an
+// What the rounding of the output o took away, rounded itself (what the products gave is then known to 2^-16 of itself in bf16, in fp16 to 2^-22, or
+// 2^-25 where that is more; the forward's cubics, 7.5e-5 of a third of P in tiles that are seen in full, are in those): 16-byte chunk c of a row, in an
 // order in which the rows of a warp are neighbours.  The backward pass needs sum_d o dO next to single dO v: where a row looks at few keys the
 // two all but cancel, and what is left of o's rounding becomes as large as dS (one key of weight 1 - w: dS is w of its parts).
 __device__ __forceinline__ long long rest_chunk(int c, int kvh, int Hkv, int rows, int n, int G, int g) {

@@ -337,9 +337,10 @@ sink_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         const int at = lane * (D / 32);  // element; a chunk has eight
         T* chunk = reinterpret_cast<T*>(p.rest + rest_chunk(at / 8, h, p.Hkv, p.rows, qs + t, p.G, hd - h * p.G));
         const float2 a = DT<T>::unpack(DT<T>::pack(x.x, x.y)), c = DT<T>::unpack(DT<T>::pack(x.z, x.w));
+        const auto lost = [](float exact, float rounded) { return isinf(exact) ? 0.f : exact - rounded; };  // (an infinity loses nothing)
         uint32_t* dst = reinterpret_cast<uint32_t*>(chunk + at % 8);
-        dst[0] = DT<T>::pack(x.x - a.x, x.y - a.y);
-        if constexpr (D == 128) dst[1] = DT<T>::pack(x.z - c.x, x.w - c.y);
+        dst[0] = DT<T>::pack(lost(x.x, a.x), lost(x.y, a.y));
+        if constexpr (D == 128) dst[1] = DT<T>::pack(lost(x.z, c.x), lost(x.w, c.y));
       }
     }
     if (staged) {

@@ -32,6 +32,13 @@ __device__ __forceinline__ float warp_dot(const float (&a)[4], const float (&b)[
   return s;
 }
 
+// 2^x.  No probability is zero where its logit is above minus infinity, however far below the smallest float: infinity times it is infinity.  (Nothing
+// finite shows the least normal number, which stands for it.)
+__device__ __forceinline__ float row_probability(float x) {
+  const float w = fast_exp2(x);
+  return w == 0.f && x > -INFINITY ? FLT_MIN : w;
+}
+
 // Output of query t (GRAD: its dQ) of query head `head`, key head `kvh`; the sequence starts at row `row0`.  lse in base 2.
 template <typename T, int D, bool GRAD>
 __device__ __noinline__ float4 exact_query_row(const SinkMaps* m, int row0, int t, int head, int kvh, int left, int sinks, float scale2,
@@ -43,10 +50,8 @@ __device__ __noinline__ float4 exact_query_row(const SinkMaps* m, int row0, int 
   for (int j = gap_at > 0 ? 0 : first; j <= t; j = j + 1 == gap_at ? first : j + 1) {
     lane_elements<T, D>(k, m->keys, (long long)(row0 + j) * m->k_sn + kvh * m->k_sh);
     lane_elements<T, D>(v, m->values, (long long)(row0 + j) * m->v_sn + kvh * m->v_sh);
-    const float x = fmaf(warp_dot(q, k), scale2, -lse);
-    float w = fast_exp2(x);
+    float w = row_probability(fmaf(warp_dot(q, k), scale2, -lse));
     if constexpr (GRAD) w *= (warp_dot(g, v) - delta) * sm_scale;
-    else if (w == 0.f && x > -INFINITY) w = FLT_MIN;  // no probability is zero: infinity times it is infinity
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, GRAD ? k[e] : v[e], acc[e]);
   }
@@ -67,7 +72,7 @@ __device__ __noinline__ void exact_key_row(float4& dk, float4& dv, const SinkMap
       lane_elements<T, D>(q, m->q, (long long)(row0 + t) * m->q_sn + head * m->q_sh);
       lane_elements<T, D>(g, m->dout, (long long)(row0 + t) * m->do_sn + head * m->do_sh);
       const float2 s = load_fresh(ld + (long long)(row0 + t) * Hq + head);
-      const float p = fast_exp2(fmaf(warp_dot(q, k), scale2, -s.x)), ds = p * (warp_dot(g, v) - s.y) * sm_scale;
+      const float p = row_probability(fmaf(warp_dot(q, k), scale2, -s.x)), ds = p * (warp_dot(g, v) - s.y) * sm_scale;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         ak[e] = fmaf(ds, q[e], ak[e]);

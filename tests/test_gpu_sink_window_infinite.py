@@ -56,3 +56,20 @@ def test_one_infinite_element(hq, hkv, d, dtype, bad, which, at):
         same = w.isfinite().all(-1) & (which in (2, 3))
         assert_within(y[same], w[same], t[same], name)
     assert device_status() == 0
+
+
+@pytest.mark.parametrize("hq,hkv", [(2, 2), (8, 1)])
+def test_gradients_by_a_probability_far_below_the_smallest_float(hq, hkv):
+    """An infinite gradient of an output reaches the value of every key that its query sees, and an infinite value the query's gradient."""
+    from native_sparse_attention_triton_b200 import ops
+
+    n, scale = 300, 3.0 / math.sqrt(128)
+    q, k, v, do = _inputs([n], hq, hkv, 128, BF, seed=9)
+    k[5] = -q[200, ::hq // hkv]  # a logit of about -130 for a query head of each group
+    do[200, 0, 7] = INF
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    o = ops.sink_window_attention(*leaves, _cu([n]), 250, 1, scale)
+    dv, = torch.autograd.grad([o], [leaves[2]], [do])
+    p = torch.softmax(q.detach()[200, 0].double() @ k.detach()[:201, 0].double().T * scale, 0)
+    assert 0 < p[5] < 1e-50
+    assert dv[:201, 0, 7].isposinf().all() and dv[5, :, :7].isfinite().all() and dv[201:].isfinite().all()

@@ -189,7 +189,7 @@ struct PairSpan {
 
 // Output of query head h * G + g of sequence b by 32-bit probabilities over the rows it sees, from its maximum m and sum l; a warp.  A row whose
 // tiles gave it a value that is not finite is computed again here: hi * inf + lo * inf is no number where lo is zero or below, nor is the product
-// of infinity and a probability that 16 or 32 bits round to zero (none is zero: at least FLT_MIN, which no finite value shows).  Some 100 clocks a
+// of infinity and a probability that 16 or 32 bits round to zero (row_probability: none is zero).  Some 100 clocks a
 // row of the cache, which only those that hold such values pay.
 template <typename T, int D>
 __device__ __noinline__ void exact_decode_row(const PagedDecodeParams* p, int b, int h, int g, float m, float l) {
@@ -206,9 +206,7 @@ __device__ __noinline__ void exact_decode_row(const PagedDecodeParams* p, int b,
       const long long pg = __shfl_sync(0xffffffffu, page, src), slot = __shfl_sync(0xffffffffu, j % p->page, src);
       lane_elements<T, D>(k, p->k, pg * p->k_sp + slot * p->k_ss + (long long)h * p->k_sh);
       lane_elements<T, D>(v, p->v, pg * p->v_sp + slot * p->v_ss + (long long)h * p->v_sh);
-      const float x = warp_dot(q, k) * p->scale2;
-      float w = fast_exp2(x - m);
-      if (w == 0.f && x > -INFINITY) w = FLT_MIN;
+      const float w = row_probability(warp_dot(q, k) * p->scale2 - m);
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, v[e], acc[e]);
     }

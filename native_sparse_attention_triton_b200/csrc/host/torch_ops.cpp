@@ -1021,6 +1021,15 @@ void check_written_pages(const Tensor& k, const Tensor& v) {
   check_written(v);
   at::assert_no_overlap(k, v);
 }
+// The stretches of memory from the tensors' first elements to their last ones meet.
+bool share_addresses(const Tensor& a, const Tensor& b) {
+  const auto end = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return static_cast<const char*>(t.data_ptr()) + (last + 1) * t.element_size();
+  };
+  return a.numel() > 0 && b.numel() > 0 && static_cast<const char*>(a.data_ptr()) < end(b) && static_cast<const char*>(b.data_ptr()) < end(a);
+}
 void wrote(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
@@ -1043,7 +1052,7 @@ Tensor paged_kv_append(const Tensor& kp, const Tensor& vp, const Tensor& table, 
   at::NoGradGuard no_grad;
   at::AutoDispatchBelowADInplaceOrView guard;
   // rows of the cache itself are read before any of it is written
-  const auto apart = [&](const Tensor& t) { return t.is_alias_of(kp) || t.is_alias_of(vp) ? t.clone(at::MemoryFormat::Contiguous) : inner_contiguous(t); };
+  const auto apart = [&](const Tensor& t) { return share_addresses(t, kp) || share_addresses(t, vp) ? t.clone(at::MemoryFormat::Contiguous) : inner_contiguous(t); };
   const Tensor k = apart(k_in), v = apart(v_in);
   Tensor after = empty({c.batch}, at::kInt, kp.device());
   if (c.batch == 0) return after;

@@ -27,3 +27,23 @@ def test_rows_of_the_cache_moved_along():
     k1[at, 10:n + 10], v1[at, 10:n + 10] = v0[at, :n], k0[at, :n]
     assert torch.equal(c.k, k1) and torch.equal(c.v, v1)
     assert device_status() == 0
+
+
+def test_rows_beside_the_cache_in_one_storage():
+    """Pages and rows cut from one buffer: nothing is copied where they do not meet."""
+    from native_sparse_attention_triton_b200 import ops
+
+    pages, rows = 4 * 16 * 2 * 128, 3 * 2 * 128
+    arena = torch.randn(2 * pages + 2 * rows, device="cuda").to(BF)
+    kp, vp = (arena[i * pages:(i + 1) * pages].view(4, 16, 2, 128) for i in range(2))
+    k, v = (arena[2 * pages + i * rows:2 * pages + (i + 1) * rows].view(3, 2, 128) for i in range(2))
+    table, held = _ints([[0], [1], [2]]), _ints([0, 5, 15])
+    k0, v0, rows_k, rows_v = kp.clone(), vp.clone(), k.clone(), v.clone()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    after = ops.paged_kv_append(kp, vp, table, held, k, v)
+    assert torch.cuda.max_memory_allocated() - before <= 512  # the lengths
+    for b, j in enumerate((0, 5, 15)):
+        k0[b, j], v0[b, j] = rows_k[b], rows_v[b]
+    assert after.tolist() == [1, 6, 16] and torch.equal(kp, k0) and torch.equal(vp, v0)
